@@ -1,0 +1,531 @@
+"""Workloads of the policy-memory operators (``mjlab_amd.seqops``): cases, inputs, plain forms and 64-bit values.
+
+``run`` computes a case with elementary torch operations in float32 (``own`` false) or through the
+framework's entry points (``own`` true). ``exact`` is the operators' definition in float64.
+
+Operators
+  scan      gated linear recurrence over a rollout (T steps, N envs, D channels) with episode resets,
+            ragged lengths and gates shared by the channels of a head; forward, or forward and backward
+  step      the recurrence's single-step form: one env step, the float32 state updated
+  norm      a residual block's epilogue and the next block's norm:
+            s = residual + scale * act(gate) * dropout(norm(y)),  n = norm(s)
+  dropout   dropout whose mask is a function of (seed, key, step counter, element index)
+"""
+
+from __future__ import annotations
+
+import math
+import sys
+from pathlib import Path
+
+import numpy as np
+import torch
+
+own = False
+
+DEVICE = "cuda"
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+SIZE = {"f32": 4, "bf16": 2, "f16": 2}
+GOLDEN = 0x9E3779B97F4A7C15
+M64 = (1 << 64) - 1
+NORM_EPS = 1e-5
+
+
+def _seqops():
+  pkg = str(Path(__file__).resolve().parents[1] / "asimov-mjlab_amd")
+  if pkg not in sys.path:
+    sys.path.insert(0, pkg)
+  from mjlab_amd import seqops
+
+  return seqops
+
+
+# ---- cases ------------------------------------------------------------------------
+def listed() -> list[dict]:
+  return [
+    # One learning iteration's rollout: 24 env steps of the G1 task's 4,096 envs, episodes ending inside it.
+    {"name": "scan_rollout", "op": "scan", "T": 24, "N": 4096, "D": 256, "G": 256, "mode": "blend", "dtype": "bf16",
+     "gate": "bf16", "resets": 0.014, "ragged": False, "envs_first": False, "train": True},
+    # A memory as wide as the policy observation (99 columns), odd sizes everywhere, float32.
+    {"name": "scan_odd", "op": "scan", "T": 37, "N": 1021, "D": 99, "G": 99, "mode": "blend", "dtype": "f32",
+     "gate": "f32", "resets": 0.05, "ragged": False, "envs_first": False, "train": True},
+    # Training on one long sequence: few rows, one float32 decay per head of 64 channels.
+    {"name": "scan_long", "op": "scan", "T": 16384, "N": 1, "D": 2048, "G": 32, "mode": "decay", "dtype": "bf16",
+     "gate": "f32", "resets": 0.0, "ragged": False, "envs_first": False, "train": True},
+    # Replaying recorded episodes of unequal lengths, stored episode by episode and padded: forward only.
+    {"name": "scan_replay", "op": "scan", "T": 4001, "N": 12, "D": 512, "G": 512, "mode": "blend", "dtype": "f16",
+     "gate": "f16", "resets": 0.0, "ragged": True, "envs_first": True, "train": False},
+    # The recurrence inside an env step of the G1 task, once per env step for all envs.
+    {"name": "step_envs", "op": "step", "N": 4096, "D": 256, "G": 256, "mode": "blend", "dtype": "bf16", "gate": "bf16",
+     "resets": 0.014},
+    # Playing a policy in one env: the smallest call, where latency counts.
+    {"name": "step_one", "op": "step", "N": 1, "D": 128, "G": 128, "mode": "blend", "dtype": "f32", "gate": "f32",
+     "resets": 0.0},
+    # The block epilogue over the same rollout, everything on, forward and backward.
+    {"name": "norm_rollout", "op": "norm", "R": 98304, "D": 256, "norm": "rms", "dtype": "bf16", "post": True, "pre": True,
+     "bias": False, "gated": True, "act": "silu", "scaled": True, "p": 0.1, "train": True},
+    # Wide rows of an odd size, layer norms with biases, no dropout.
+    {"name": "norm_wide", "op": "norm", "R": 2047, "D": 4097, "norm": "layer", "dtype": "f32", "post": True, "pre": True,
+     "bias": True, "gated": True, "act": "sigmoid", "scaled": True, "p": 0.0, "train": True},
+    # The plain pre-norm residual block of a long sequence (no gate, no scale).
+    {"name": "norm_plain", "op": "norm", "R": 16384, "D": 2048, "norm": "rms", "dtype": "bf16", "post": False, "pre": True,
+     "bias": False, "gated": False, "act": "silu", "scaled": False, "p": 0.0, "train": True},
+    # The epilogue inside an env step: a handful of rows, forward only.
+    {"name": "norm_step", "op": "norm", "R": 16, "D": 1000, "norm": "rms", "dtype": "f16", "post": True, "pre": True,
+     "bias": False, "gated": True, "act": "silu", "scaled": True, "p": 0.0, "train": False},
+    # Sensor dropout on the policy observation of all envs (values kept unscaled).
+    {"name": "dropout_obs", "op": "dropout", "R": 4096, "D": 99, "dtype": "f32", "p": 0.05, "rescale": False, "train": False},
+    # Dropout on a rollout's activations, forward and backward.
+    {"name": "dropout_rollout", "op": "dropout", "R": 98304, "D": 512, "dtype": "bf16", "p": 0.1, "rescale": True,
+     "train": True},
+  ]
+
+
+def _log_int(rng, lo: int, hi: int) -> int:
+  return max(lo, min(hi, round(math.exp(rng.uniform(math.log(lo), math.log(hi))))))
+
+
+def draw(rng) -> dict:
+  """One more case: every operator, type and option of the listed ones, sizes over their logarithms."""
+  most = max(work(c)["bytes"] for c in listed())
+  while True:
+    op = rng.choice(["scan", "scan", "step", "norm", "norm", "dropout"])
+    dtype = rng.choice(["f32", "bf16", "f16"])
+    if op in ("scan", "step"):
+      heads = rng.random() < 0.4
+      if heads:
+        g, k = _log_int(rng, 1, 32), _log_int(rng, 2, 256)
+      else:
+        g, k = _log_int(rng, 1, 4096), 1
+      c = {"op": op, "N": _log_int(rng, 1, 8192), "D": g * k, "G": g, "mode": rng.choice(["blend", "decay"]), "dtype": dtype,
+           "gate": rng.choice([dtype, "f32"]), "resets": rng.choice([0.0, 0.01, 0.2])}
+      if op == "scan":
+        c.update(T=_log_int(rng, 1, 16384), ragged=rng.random() < 0.3, envs_first=rng.random() < 0.5, train=rng.random() < 0.6)
+      elems = c["N"] * c["D"] * c.get("T", 1)
+    elif op == "norm":
+      c = {"op": op, "R": _log_int(rng, 1, 131072), "D": _log_int(rng, 2, 8192), "norm": rng.choice(["rms", "layer"]),
+           "dtype": dtype, "post": rng.random() < 0.7, "pre": rng.random() < 0.8, "bias": rng.random() < 0.4,
+           "gated": rng.random() < 0.6, "act": rng.choice(["silu", "sigmoid"]), "scaled": rng.random() < 0.6,
+           "p": rng.choice([0.0, 0.1, 0.5]), "train": rng.random() < 0.6}
+      elems = c["R"] * c["D"]
+    else:
+      c = {"op": op, "R": _log_int(rng, 1, 131072), "D": _log_int(rng, 1, 4096), "dtype": dtype,
+           "p": rng.choice([0.01, 0.1, 0.5]), "rescale": rng.random() < 0.7, "train": rng.random() < 0.5}
+      elems = c["R"] * c["D"]
+    if elems >= 64 and work(c)["bytes"] <= most and elems <= 50_331_648:
+      return c
+
+
+def work(case: dict) -> dict:
+  """Each input read once and each output written once, and the definition's operations."""
+  b = SIZE[case["dtype"]]
+  if case["op"] in ("scan", "step"):
+    n, d, g, t = case["N"], case["D"], case["G"], case.get("T", 1)
+    x, gate, state = t * n * d * b, t * n * g * SIZE[case["gate"]], n * d * 4
+    reset = t * n if case["resets"] else 0
+    if case.get("train"):
+      return {"bytes": 4 * x + 2 * gate + 4 * state + reset, "flops": 16 * t * n * d}
+    return {"bytes": 2 * x + gate + 2 * state + reset, "flops": 4 * t * n * d}
+  e = case["R"] * case["D"]
+  if case["op"] == "dropout":
+    return {"bytes": e * b * (4 if case["train"] else 2), "flops": e * (2 if case["train"] else 1)}
+  ins = 2 + case["gated"]
+  outs = 1 + case["pre"]
+  if case["train"]:
+    ins, outs = ins + 1 + case["pre"], outs + 2 + case["gated"]
+  per = 4 + 6 * case["post"] + 6 * case["pre"] + 6 * case["gated"]
+  return {"bytes": e * b * (ins + outs), "flops": e * per * (3 if case["train"] else 1)}
+
+
+# ---- inputs -----------------------------------------------------------------------
+def prepare(case: dict, seed: int) -> dict:
+  gen = torch.Generator(device=DEVICE)
+  gen.manual_seed(seed)
+  dt = TYPES[case["dtype"]]
+
+  def normal(*shape):
+    return torch.randn(*shape, generator=gen, device=DEVICE)
+
+  st = {"case": case}
+  if case["op"] in ("scan", "step"):
+    n, d, g, t, k = case["N"], case["D"], case["G"], case.get("T", 1), case["D"] // case["G"]
+    lead = (n, t) if case.get("envs_first") else (t, n)
+
+    def seq(v):  # time-major view; episode-major storage where the case says so
+      return v.transpose(0, 1) if case.get("envs_first") else v
+
+    x = normal(*lead, d).to(dt)
+    if case["mode"] == "blend":
+      gate = normal(*lead, g) * 1.5 + 1.5
+    else:  # decays of 2 to 2000 steps
+      rate = torch.exp(torch.rand(g, generator=gen, device=DEVICE) * 6.9 - 7.6)
+      gate = torch.exp(-rate * torch.nn.functional.softplus(normal(*lead, g)))
+    gate = gate.to(TYPES[case["gate"]])
+    st["state"] = normal(n, d)
+    st["x"], st["gate"] = seq(x), seq(gate)
+    st["reset"] = (torch.rand(t, n, generator=gen, device=DEVICE) < case["resets"]) if case["resets"] else None
+    st["lengths"] = (torch.randint(0, t + 1, (n,), generator=gen, device=DEVICE, dtype=torch.int32)
+                     if case.get("ragged") else None)
+    if case["op"] == "step":
+      st.update(x=st["x"][0], gate=st["gate"][0], reset=None if st["reset"] is None else st["reset"][0])
+      st["next"] = torch.empty_like(st["state"])  # the program swaps the two state buffers every env step
+    elif case["train"]:
+      st["dh"], st["dstate"] = seq(normal(*lead, d).to(dt)), normal(n, d)
+      for name in ("x", "gate", "state"):
+        st[name].requires_grad_(True)
+    return st
+  r, d = case["R"], case["D"]
+  st["seed"], st["key"] = (seed * GOLDEN) & M64, (0xD1B54A32D192ED03 ^ seed) & M64
+  st["ctr"] = torch.tensor([seed % 1000 + 1], dtype=torch.int64, device=DEVICE)
+  if case["op"] == "dropout":
+    st["x"] = normal(r, d).to(dt)
+    if case["train"]:
+      st["dy"] = normal(r, d).to(dt)
+      st["x"].requires_grad_(True)
+    return st
+  st["y"] = (normal(r, d) * 2).to(dt)
+  st["res"] = (normal(r, d) * 3).to(dt)
+  st["gate"] = normal(r, d).to(dt) if case["gated"] else None
+  st["scale"] = 0.1 + 0.02 * normal(d) if case["scaled"] else None
+  for side in ("post", "pre"):
+    st[side + "_w"] = 1 + 0.1 * normal(d) if case[side] else None
+    st[side + "_b"] = 0.1 * normal(d) if case[side] and case["bias"] else None
+  if case["train"]:
+    st["ds"] = normal(r, d).to(dt)
+    st["dn"] = normal(r, d).to(dt) if case["pre"] else None
+    for name in NORM_LEAVES:
+      if st[name] is not None:
+        st[name].requires_grad_(True)
+  return st
+
+
+NORM_LEAVES = ("y", "res", "gate", "scale", "post_w", "post_b", "pre_w", "pre_b")
+
+
+def run(state: dict):
+  return (_own if own else _plain)(state)
+
+
+# ---- the framework's entry points ------------------------------------------------
+def _own(st: dict):
+  ops = _seqops()
+  case = st["case"]
+  if case["op"] == "step":
+    return list(ops.gated_step(st["x"], st["gate"], st["state"], st["reset"], mode=case["mode"], out=st["next"]))
+  if case["op"] == "scan":
+    h, last = ops.gated_scan(st["x"], st["gate"], st["state"], st["reset"], st["lengths"], mode=case["mode"])
+    if not case["train"]:
+      return [h, last]
+    grads = torch.autograd.grad([h, last], [st["x"], st["gate"], st["state"]], [st["dh"], st["dstate"]])
+    return [h.detach(), last.detach(), *grads]
+  if case["op"] == "dropout":
+    scale = None if case["rescale"] else 1.0
+    y = ops.dropout(st["x"], case["p"], st["seed"], st["key"], st["ctr"], scale=scale)
+    if not case["train"]:
+      return [y]
+    return [y.detach(), *torch.autograd.grad(y, st["x"], st["dy"])]
+  s, n = ops.residual_norm(st["y"], st["res"], pre_weight=st["pre_w"], pre_bias=st["pre_b"], post_weight=st["post_w"],
+                           post_bias=st["post_b"], gate=st["gate"], act=case["act"], scale=st["scale"], norm=case["norm"],
+                           eps=NORM_EPS, p=case["p"], seed=st["seed"], key=st["key"], ctr=st["ctr"])
+  outs = [s] if n is None else [s, n]
+  if not case["train"]:
+    return outs
+  leaves = [st[name] for name in NORM_LEAVES if st[name] is not None]
+  grads = torch.autograd.grad(outs, leaves, [st["ds"]] if n is None else [st["ds"], st["dn"]])
+  return [o.detach() for o in outs] + list(grads)
+
+
+# ---- plain forms --------------------------------------------------------------------
+def _plain(st: dict):
+  with torch.no_grad():
+    return {"scan": _plain_scan, "step": _plain_step, "norm": _plain_norm, "dropout": _plain_dropout}[st["case"]["op"]](st)
+
+
+def _linear_scan(a: torch.Tensor, b: torch.Tensor, h0: torch.Tensor) -> torch.Tensor:
+  """h_t = a_t h_{t-1} + b_t along dim 0; long sequences in blocks of about sqrt(T) steps, all blocks at once."""
+  t, n, d = b.shape
+  a = a.expand(t, n, d)
+  if t <= 64:
+    out, h = torch.empty_like(b), h0
+    for i in range(t):
+      h = a[i] * h + b[i]
+      out[i] = h
+    return out
+  width = math.isqrt(t - 1) + 1
+  blocks = -(-t // width)
+  pad = blocks * width - t
+  a = torch.cat([a, a.new_ones(pad, n, d)]).view(blocks, width, n, d)
+  b = torch.cat([b, b.new_zeros(pad, n, d)]).view(blocks, width, n, d)
+  prod, part = torch.empty_like(b), torch.empty_like(b)
+  pa, pb = torch.ones_like(b[:, 0]), torch.zeros_like(b[:, 0])
+  for i in range(width):
+    pa, pb = a[:, i] * pa, a[:, i] * pb + b[:, i]
+    prod[:, i], part[:, i] = pa, pb
+  starts, h = torch.empty_like(pa), h0
+  for j in range(blocks):
+    starts[j] = h
+    h = prod[j, -1] * h + part[j, -1]
+  return (prod * starts[:, None] + part).view(blocks * width, n, d)[:t]
+
+
+def _gates(st: dict, t: int, n: int, d: int):
+  """(a, 1 - a, inside) in float32, per channel; inside is None or the (T, N, 1) steps before each row's length."""
+  case = st["case"]
+  g = st["gate"].float().reshape(t, n, -1)
+  g = g if g.shape[2] == d else g.repeat_interleave(d // g.shape[2], dim=2)
+  if case["mode"] == "blend":
+    a, rest = torch.sigmoid(g), torch.sigmoid(-g)
+  else:
+    a, rest = g, None
+  inside = None
+  if st.get("lengths") is not None:
+    inside = torch.arange(t, device=DEVICE)[:, None, None] < st["lengths"][None, :, None]
+  return a, rest, inside
+
+
+def _plain_scan(st: dict):
+  case = st["case"]
+  x = st["x"]
+  t, n, d = x.shape
+  dt, gt = x.dtype, st["gate"].dtype
+  xf = x.float()
+  a, rest, inside = _gates(st, t, n, d)
+  b = xf if rest is None else rest * xf
+  carry = a  # the factor of the previous state
+  if st["reset"] is not None:
+    carry = torch.where(st["reset"][:, :, None], 0.0, carry)
+  if inside is not None:
+    carry, b = torch.where(inside, carry, 1.0), torch.where(inside, b, 0.0)
+  h0 = st["state"].float()
+  h = _linear_scan(carry, b, h0)
+  last = h[-1].clone()
+  shown = h if inside is None else torch.where(inside, h, 0.0)
+  if not case["train"]:
+    return [shown.to(dt), last]
+  dh = st["dh"].float()
+  if inside is not None:
+    dh = torch.where(inside, dh, 0.0)
+  after = torch.cat([carry[1:], torch.ones_like(carry[:1])])  # delta_t = dh_t + carry_{t+1} delta_{t+1}
+  delta = _linear_scan(after.flip(0), dh.flip(0), st["dstate"].float()).flip(0)
+  before = torch.cat([h0[None], h[:-1]])
+  if st["reset"] is not None:
+    before = torch.where(st["reset"][:, :, None], 0.0, before)
+  if rest is None:
+    dx, dg = delta, delta * before
+  else:
+    dx, dg = rest * delta, delta * (before - xf) * a * rest
+  if inside is not None:
+    dx, dg = torch.where(inside, dx, 0.0), torch.where(inside, dg, 0.0)
+  dg = dg.view(t, n, case["G"], -1).sum(-1)
+  return [shown.to(dt), last, dx.to(dt), dg.to(gt), carry[0] * delta[0]]
+
+
+def _plain_step(st: dict):
+  x = st["x"]
+  n, d = x.shape
+  a, rest, _ = _gates(st, 1, n, d)
+  prev = st["state"]
+  if st["reset"] is not None:
+    prev = torch.where(st["reset"][:, None], 0.0, prev)
+  xf = x.float()
+  h = a[0] * prev + (xf if rest is None else rest[0] * xf)
+  return [h.to(x.dtype), h]
+
+
+def _shift(z: torch.Tensor, k: int) -> torch.Tensor:
+  return (z >> k) & ((1 << (64 - k)) - 1)  # a logical shift of 64-bit words
+
+
+def _signed(v: int) -> int:
+  return v - (1 << 64) if v >> 63 else v
+
+
+def _mix(z: torch.Tensor) -> torch.Tensor:
+  z = (z ^ _shift(z, 30)) * _signed(0xBF58476D1CE4E5B9)
+  z = (z ^ _shift(z, 27)) * _signed(0x94D049BB133111EB)
+  return z ^ _shift(z, 31)
+
+
+def _kept(st: dict, r: int, d: int) -> torch.Tensor:
+  """The (R, D) keep mask: element i takes half of the 64-bit word i // 2 of the (seed, key, counter) stream."""
+  base = _mix(_signed(st["seed"]) ^ _mix(_signed(st["key"]) ^ _mix(st["ctr"] + _signed(GOLDEN))))
+  i = torch.arange(r * d, device=DEVICE, dtype=torch.int64)
+  z = _mix(base + (_shift(i, 1) + 1) * _signed(GOLDEN))
+  bits = torch.where((i & 1) == 0, _shift(z, 32), z & 0xFFFFFFFF)
+  return (bits >= round(st["case"]["p"] * (1 << 32))).view(r, d)
+
+
+def _plain_dropout(st: dict):
+  case, x = st["case"], st["x"]
+  keep = _kept(st, *x.shape)
+  scale = 1.0 / (1.0 - case["p"]) if case["rescale"] else 1.0
+  outs = [torch.where(keep, x.float() * scale, 0.0).to(x.dtype)]
+  if case["train"]:
+    outs.append(torch.where(keep, st["dy"].float() * scale, 0.0).to(x.dtype))
+  return outs
+
+
+def _normed(v: torch.Tensor, kind: str):
+  """(normalised rows, 1 / deviation)."""
+  if kind == "layer":
+    v = v - v.mean(1, keepdim=True)
+  inv = 1.0 / torch.sqrt((v * v).mean(1, keepdim=True) + NORM_EPS)
+  return v * inv, inv
+
+
+def _norm_grad(dv: torch.Tensor, hat: torch.Tensor, inv: torch.Tensor, kind: str) -> torch.Tensor:
+  out = dv - hat * (dv * hat).mean(1, keepdim=True)
+  if kind == "layer":
+    out = out - dv.mean(1, keepdim=True)
+  return out * inv
+
+
+def _plain_norm(st: dict):
+  case, dt = st["case"], st["y"].dtype
+  kind, r, d = case["norm"], case["R"], case["D"]
+  v = st["y"].float()
+  if case["post"]:
+    yhat, yinv = _normed(v, kind)
+    v = yhat * st["post_w"]
+    if st["post_b"] is not None:
+      v = v + st["post_b"]
+  keep = None
+  if case["p"] > 0:
+    keep = _kept(st, r, d).float() / (1.0 - case["p"])
+  u = v if keep is None else v * keep
+  act = None
+  if case["gated"]:
+    g = st["gate"].float()
+    sig = torch.sigmoid(g)
+    act = sig * g if case["act"] == "silu" else sig
+  scale = st["scale"]
+  w = u if act is None else act * u
+  s = st["res"].float() + (w if scale is None else scale * w)
+  outs = [s.to(dt)]
+  if case["pre"]:
+    shat, sinv = _normed(s, kind)
+    outs.append((shat * st["pre_w"] + (0.0 if st["pre_b"] is None else st["pre_b"])).to(dt))
+  if not case["train"]:
+    return outs
+  ds = st["ds"].float()
+  if case["pre"]:
+    dn = st["dn"].float()
+    ds = ds + _norm_grad(dn * st["pre_w"], shat, sinv, kind)
+  grads = {"res": ds.to(dt)}
+  if case["pre"]:
+    grads["pre_w"] = (dn * shat).sum(0)
+    if st["pre_b"] is not None:
+      grads["pre_b"] = dn.sum(0)
+  dw = ds
+  if scale is not None:
+    grads["scale"] = (ds * w).sum(0)
+    dw = ds * scale
+  if act is not None:
+    slope = sig * (1.0 - sig) if case["act"] == "sigmoid" else sig * (1.0 + g * (1.0 - sig))
+    grads["gate"] = (dw * u * slope).to(dt)
+    dw = dw * act
+  dv = dw if keep is None else dw * keep
+  if case["post"]:
+    grads["post_w"] = (dv * yhat).sum(0)
+    if st["post_b"] is not None:
+      grads["post_b"] = dv.sum(0)
+    dv = _norm_grad(dv * st["post_w"], yhat, yinv, kind)
+  grads["y"] = dv.to(dt)
+  return outs + [grads[name] for name in NORM_LEAVES if name in grads]
+
+
+# ---- the definition in 64 bits -------------------------------------------------------
+def exact(case: dict, seed: int):
+  st = prepare(case, seed)
+  lead = {k: v.detach().double() for k, v in st.items() if torch.is_tensor(v) and v.is_floating_point()}
+  if case["op"] == "dropout":
+    keep = torch.from_numpy(_kept_words(st, case["R"] * case["D"], case["p"])).to(DEVICE).view(case["R"], case["D"])
+    k = 1.0 / (1.0 - case["p"]) if case["rescale"] else 1.0
+    return [torch.where(keep, lead[n] * k, 0.0) for n in (("x", "dy") if case["train"] else ("x",))]
+  if case["op"] == "norm":
+    return _exact_norm(case, st, lead)
+  return _exact_scan(case, st, lead)
+
+
+def _kept_words(st: dict, count: int, p: float) -> np.ndarray:
+  def mix_int(z):
+    z = ((z ^ (z >> 30)) * 0xBF58476D1CE4E5B9) & M64
+    z = ((z ^ (z >> 27)) * 0x94D049BB133111EB) & M64
+    return z ^ (z >> 31)
+
+  base = mix_int(st["seed"] ^ mix_int(st["key"] ^ mix_int((int(st["ctr"][0]) + GOLDEN) & M64)))
+  z = np.arange(1, (count + 1) // 2 + 1, dtype=np.uint64) * np.uint64(GOLDEN) + np.uint64(base)
+  z = (z ^ (z >> np.uint64(30))) * np.uint64(0xBF58476D1CE4E5B9)
+  z = (z ^ (z >> np.uint64(27))) * np.uint64(0x94D049BB133111EB)
+  z = z ^ (z >> np.uint64(31))
+  bits = np.stack([z >> np.uint64(32), z & np.uint64(0xFFFFFFFF)], axis=1).reshape(-1)[:count]
+  return bits >= np.uint64(round(p * (1 << 32)))
+
+
+def _exact_scan(case: dict, st: dict, v: dict):
+  """The recurrence step by step; gradients by differentiating it in float64."""
+  step = case["op"] == "step"
+  x, gate = (v["x"][None], v["gate"][None]) if step else (v["x"], v["gate"])
+  t, n, d = x.shape
+  leaves = [x, gate, v["state"]]
+  train = bool(case.get("train"))
+  for leaf in leaves:
+    leaf.requires_grad_(train)
+  with torch.set_grad_enabled(train):
+    h, rows = leaves[2], []
+    full = gate[..., None].expand(t, n, case["G"], d // case["G"]).reshape(t, n, d)
+    # one op for all steps, so that its gradient is one op too
+    decay = torch.sigmoid(full) if case["mode"] == "blend" else full
+    added = torch.sigmoid(-full) * x if case["mode"] == "blend" else x
+    reset = st["reset"][None] if step and st["reset"] is not None else st["reset"]
+    lengths = st.get("lengths")
+    for decay_t, added_t, i in zip(decay.unbind(0), added.unbind(0), range(t)):
+      new = h
+      if reset is not None:
+        new = new.masked_fill(reset[i][:, None], 0.0)
+      new = torch.addcmul(added_t, decay_t, new)
+      if lengths is None:
+        h = new
+        rows.append(h)
+      else:
+        live = (i < lengths)[:, None]
+        h = torch.where(live, new, h)
+        rows.append(new.masked_fill(~live, 0.0))
+    if step:
+      return [rows[0].detach(), h.detach()]
+    hs = torch.stack(rows)
+  if not train:
+    return [hs, h]
+  grads = torch.autograd.grad([hs, h], leaves, [v["dh"], v["dstate"]])
+  return [hs.detach(), h.detach(), *grads]
+
+
+def _exact_norm(case: dict, st: dict, v: dict):
+  r, d = case["R"], case["D"]
+  present = [name for name in NORM_LEAVES if st[name] is not None]
+  leaves = [v[name].requires_grad_(case["train"]) for name in present]
+
+  def norm(z, w, b):
+    mean = z.mean(1, keepdim=True) if case["norm"] == "layer" else 0.0
+    var = ((z - mean) ** 2).mean(1, keepdim=True)
+    out = (z - mean) / torch.sqrt(var + NORM_EPS) * w
+    return out if b is None else out + b
+
+  with torch.set_grad_enabled(case["train"]):
+    block = v["y"]
+    if case["post"]:
+      block = norm(block, v["post_w"], v.get("post_b"))
+    if case["p"] > 0:
+      keep = torch.from_numpy(_kept_words(st, r * d, case["p"])).to(DEVICE).view(r, d)
+      block = torch.where(keep, block / (1.0 - case["p"]), 0.0)
+    if case["gated"]:
+      block = block * torch.sigmoid(v["gate"]) * (v["gate"] if case["act"] == "silu" else 1.0)
+    if case["scaled"]:
+      block = block * v["scale"]
+    outs = [v["res"] + block]
+    if case["pre"]:
+      outs.append(norm(outs[0], v["pre_w"], v.get("pre_b")))
+  if not case["train"]:
+    return outs
+  grads = torch.autograd.grad(outs, leaves, [v["ds"]] + ([v["dn"]] if case["pre"] else []))
+  return [o.detach() for o in outs] + list(grads)
