@@ -102,6 +102,18 @@ EXPORTS = (
   "mjh_time_out",
   "mjh_masked_copy",
   "mjh_masked_zero_i64",
+  "mjh_sizeof_scan_desc",
+  "mjh_sizeof_resnorm_desc",
+  "mjh_seq_last_error",
+  "mjh_scan_steps",
+  "mjh_scan_workspace",
+  "mjh_scan_forward",
+  "mjh_scan_backward",
+  "mjh_scan_step",
+  "mjh_resnorm_workspace",
+  "mjh_resnorm_forward",
+  "mjh_resnorm_backward",
+  "mjh_dropout",
 )
 
 
@@ -214,6 +226,14 @@ def lib() -> ctypes.CDLL:
   L.mjh_motion_frame.argtypes = [vp, vp, vp, ci, ci, ci, vp, vp, ll, ll, vp]
   L.mjh_motion_reset.argtypes = [vp, ll, ci, ci, ci, ci, ci, vp, ll, vp, vp, vp, vp, vp, ci, ci, cf, cf, vp, ll, vp, ll, ci, ci,
                                  vp, ll, ci, ci, u64, u64, vp, ll, vp]
+  L.mjh_sizeof_scan_desc.restype = L.mjh_sizeof_resnorm_desc.restype = ctypes.c_size_t
+  L.mjh_seq_last_error.restype = ctypes.c_char_p
+  L.mjh_scan_workspace.argtypes = [vp, ci]
+  L.mjh_resnorm_workspace.argtypes = [vp]
+  L.mjh_scan_workspace.restype = L.mjh_resnorm_workspace.restype = ll
+  for f in (L.mjh_scan_forward, L.mjh_scan_backward, L.mjh_scan_step, L.mjh_resnorm_forward, L.mjh_resnorm_backward):
+    f.argtypes = [vp, vp]
+  L.mjh_dropout.argtypes = [vp, ll, vp, ll, ll, ci, ci, cf, u64, u64, u64, vp, vp, vp]
   if L.mjh_abi_version() != ABI_VERSION:
     raise NativeLibraryError(f"libmjh ABI {L.mjh_abi_version()} != {ABI_VERSION}")
   if L.mjh_sizeof_model() != ctypes.sizeof(abi.model_struct()):

@@ -618,6 +618,143 @@ int mjh_reset_stats(const unsigned char* reset, unsigned char* any_reset, mjh_i6
 int mjh_event_mark(int* last, unsigned char* once, const unsigned char* mask, const mjh_i64* step, long long n,
                    void* stream);
 
+/* ---- policy memory (mjh_scan.hip, mjh_resnorm.hip) ----
+ * What a policy with a memory runs per env step and over a rollout: a gated
+ * linear recurrence whose state is cleared at episode ends, a residual block's
+ * epilogue fused with the next block's norm, and dropout. Their counterpart in
+ * the reference is the learner's network (rl_cfg.py:12-21, an MLP without memory).
+ * Element types: MJH_F32, MJH_BF16, MJH_F16; strides count elements, the last
+ * dimension's is 1. Statistics, states and sums are float32. Nothing allocates
+ * or synchronises; workspaces are the caller's and are free again when the
+ * launch has run. Return codes: 0, 1 (refused, mjh_seq_last_error says why), 2
+ * (launch failed). */
+#define MJH_F32 0
+#define MJH_BF16 1
+#define MJH_F16 2
+
+#define MJH_SCAN_DECAY 0 /* h = gate h' + x */
+#define MJH_SCAN_BLEND 1 /* h = sigmoid(gate) h' + sigmoid(-gate) x */
+
+#define MJH_ACT_SILU 0
+#define MJH_ACT_SIGMOID 1
+
+/* x (T, N, D), gate (T, N, G) with G dividing D (channel d uses gate d / (D / G)),
+ * reset (T, N) bytes or NULL (non-zero: the state before the step is 0), lengths
+ * (N) or NULL (steps from lengths[n] on leave the state and output 0), state and
+ * last (N, D) contiguous, state NULL = 0. kept: (ceil(T / mjh_scan_steps()), N, D)
+ * float32, written by the forward pass when not NULL, read by the backward pass.
+ * Backward: dh (T, N, D) or NULL = 0, dlast (N, D) or NULL = 0; dx, dgate, dstate
+ * NULL = not wanted. gtype: dtype or MJH_F32. */
+typedef struct mjh_scan_desc {
+  const void* x;
+  long long xt, xn;
+  const void* gate;
+  long long gt, gn;
+  const float* state;
+  const unsigned char* reset;
+  long long rt, rn;
+  const int* lengths;
+  void* h;
+  long long ht, hn;
+  float* last;
+  float* kept;
+  const void* dh;
+  long long dht, dhn;
+  const float* dlast;
+  void* dx;
+  long long dxt, dxn;
+  void* dgate;
+  long long dgt, dgn;
+  float* dstate;
+  void* ws;
+  long long ws_bytes;
+  int T, N, D, G;
+  int dtype, gtype, mode;
+} mjh_scan_desc;
+
+size_t mjh_sizeof_scan_desc(void);
+size_t mjh_sizeof_resnorm_desc(void);
+
+/* The last refusal of a call of this section on this thread. */
+const char* mjh_seq_last_error(void);
+
+/* Steps between the states that the forward pass keeps for the backward pass. */
+int mjh_scan_steps(void);
+
+/* Bytes of workspace for one forward (backward != 0: backward) call; -1: refused. */
+long long mjh_scan_workspace(const mjh_scan_desc* d, int backward);
+
+int mjh_scan_forward(const mjh_scan_desc* d, void* stream);
+int mjh_scan_backward(const mjh_scan_desc* d, void* stream);
+
+/* T = 1 for serving: last = the state after the step (may be state itself). */
+int mjh_scan_step(const mjh_scan_desc* d, void* stream);
+
+/* R rows of D <= 8192 columns at row strides *s:
+ *   p = norm(y) (post != 0: rms or, layer != 0, layer norm with post_w / post_b), or y
+ *   u = dropout(p) (thr = round(prob 2^32); 0 = none; element index row * D + column)
+ *   s = r + scale * act(gate) * u       n = norm(s) (pre != 0, pre_w / pre_b)
+ * y NULL: s = r (not written). gate, scale, the weights and biases may be NULL. scale: D
+ * values, or one when scale_one != 0. w32: weights, biases and scale are float32,
+ * else dtype. stats (R, 4) float32, 16-byte aligned: written by the forward pass when
+ * not NULL, read by the backward pass. ctr_out: receives *ctr (the backward pass
+ * takes that copy as its ctr). Backward: ds / dn NULL = 0; outputs NULL = not wanted. */
+typedef struct mjh_resnorm_desc {
+  const void* y;
+  long long ys;
+  const void* r;
+  long long rs;
+  const void* gate;
+  long long gs;
+  const void* post_w;
+  const void* post_b;
+  const void* pre_w;
+  const void* pre_b;
+  const void* scale;
+  void* s;
+  long long ss;
+  void* n;
+  long long ns;
+  float* stats;
+  const void* ds;
+  long long dss;
+  const void* dn;
+  long long dns;
+  void* dy;
+  long long dys;
+  void* dr;
+  long long drs;
+  void* dgate;
+  long long dgs;
+  void* d_post_w;
+  void* d_post_b;
+  void* d_pre_w;
+  void* d_pre_b;
+  void* d_scale;
+  void* ws;
+  long long ws_bytes;
+  long long R;
+  unsigned long long thr, seed, key;
+  const mjh_i64* ctr;
+  mjh_i64* ctr_out;
+  int D, dtype, w32, scale_one;
+  int layer, act, post, pre;
+  float eps, drop_scale;
+} mjh_resnorm_desc;
+
+long long mjh_resnorm_workspace(const mjh_resnorm_desc* d);
+int mjh_resnorm_forward(const mjh_resnorm_desc* d, void* stream);
+int mjh_resnorm_backward(const mjh_resnorm_desc* d, void* stream);
+
+/* y = keep ? x * scale : 0 for rows x cols elements (row strides xs, ys). Element
+ * i = row * cols + column takes the high (even i) or low half of word i / 2 of the
+ * (seed, key, *ctr) stream: word w = mix(base + (w + 1) 0x9e3779b97f4a7c15), base and
+ * mix as for mjh_uniform_draws; it is kept iff those 32 bits are >= thr. The
+ * gradient is the same call on dy with ctr = the ctr_out of the forward call. */
+int mjh_dropout(const void* x, long long xs, void* y, long long ys, long long rows, int cols, int dtype, float scale,
+                unsigned long long thr, unsigned long long seed, unsigned long long key, const mjh_i64* ctr,
+                mjh_i64* ctr_out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

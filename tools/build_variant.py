@@ -21,7 +21,8 @@ name, flags = sys.argv[1], sys.argv[2:]
 OUTD.mkdir(parents=True, exist_ok=True)
 tmp = Path("/tmp/mjh_variants") / name
 tmp.mkdir(parents=True, exist_ok=True)
-srcs = [CSRC / f for f in ("mjh_step.hip", "mjh_envops.hip", "mjh_mdp.hip", "mjh_mgr.hip", "mjh_fuse.hip")]
+srcs = [CSRC / f for f in ("mjh_step.hip", "mjh_envops.hip", "mjh_mdp.hip", "mjh_mgr.hip", "mjh_fuse.hip", "mjh_scan.hip",
+                           "mjh_resnorm.hip")]
 if os.environ.get("MJH_STEP_SRC"):  # A/B against another revision of the step kernel (e.g. a saved HEAD copy)
   srcs[0] = Path(os.environ["MJH_STEP_SRC"])
 
