@@ -14,6 +14,7 @@ Operators
 
 from __future__ import annotations
 
+import functools
 import math
 import sys
 from pathlib import Path
@@ -31,10 +32,10 @@ M64 = (1 << 64) - 1
 NORM_EPS = 1e-5
 
 
+@functools.cache
 def _seqops():
-  pkg = str(Path(__file__).resolve().parents[1] / "asimov-mjlab_amd")
-  if pkg not in sys.path:
-    sys.path.insert(0, pkg)
+  """The framework's operators, imported once as a program does (not looked up at every call)."""
+  sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "asimov-mjlab_amd"))
   from mjlab_amd import seqops
 
   return seqops
