@@ -8,6 +8,8 @@ the output's type."""
 
 from __future__ import annotations
 
+import ctypes
+
 import numpy as np
 import torch
 
@@ -178,3 +180,29 @@ def resnorm(y, r, gate=None, scale=None, post_w=None, post_b=None, pre_w=None, p
     dp, mdp = back(dp * post_w, mdp * post_w.abs(), hat, mhat, rstd, kappa)
   out["y"] = (dp, mdp)
   return out
+
+
+# ---- the C descriptors (include/mjh_abi.h), for calls of the entry points themselves ----
+_vp, _ll, _ci, _u64, _cf = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int, ctypes.c_ulonglong, ctypes.c_float
+
+
+class ScanDesc(ctypes.Structure):
+  """``mjh_scan_desc`` (include/mjh_abi.h)."""
+
+  _fields_ = [("x", _vp), ("xt", _ll), ("xn", _ll), ("gate", _vp), ("gt", _ll), ("gn", _ll), ("state", _vp), ("reset", _vp),
+              ("rt", _ll), ("rn", _ll), ("lengths", _vp), ("h", _vp), ("ht", _ll), ("hn", _ll), ("last", _vp), ("kept", _vp),
+              ("dh", _vp), ("dht", _ll), ("dhn", _ll), ("dlast", _vp), ("dx", _vp), ("dxt", _ll), ("dxn", _ll),
+              ("dgate", _vp), ("dgt", _ll), ("dgn", _ll), ("dstate", _vp), ("ws", _vp), ("ws_bytes", _ll), ("T", _ci),
+              ("N", _ci), ("D", _ci), ("G", _ci), ("dtype", _ci), ("gtype", _ci), ("mode", _ci)]
+
+
+class ResnormDesc(ctypes.Structure):
+  """``mjh_resnorm_desc`` (include/mjh_abi.h)."""
+
+  _fields_ = [("y", _vp), ("ys", _ll), ("r", _vp), ("rs", _ll), ("gate", _vp), ("gs", _ll), ("post_w", _vp), ("post_b", _vp),
+              ("pre_w", _vp), ("pre_b", _vp), ("scale", _vp), ("s", _vp), ("ss", _ll), ("n", _vp), ("ns", _ll),
+              ("stats", _vp), ("ds", _vp), ("dss", _ll), ("dn", _vp), ("dns", _ll), ("dy", _vp), ("dys", _ll), ("dr", _vp),
+              ("drs", _ll), ("dgate", _vp), ("dgs", _ll), ("d_post_w", _vp), ("d_post_b", _vp), ("d_pre_w", _vp),
+              ("d_pre_b", _vp), ("d_scale", _vp), ("ws", _vp), ("ws_bytes", _ll), ("R", _ll), ("thr", _u64), ("seed", _u64),
+              ("key", _u64), ("ctr", _vp), ("ctr_out", _vp), ("D", _ci), ("dtype", _ci), ("w32", _ci), ("scale_one", _ci),
+              ("layer", _ci), ("act", _ci), ("post", _ci), ("pre", _ci), ("eps", _cf), ("drop_scale", _cf)]

@@ -205,7 +205,7 @@ def test_dropout_refusals(kw, match):
 def _scan_desc(**kw):
   """A host-side description; only sizes, types, strides and pointer alignment are looked at."""
   buf = torch.zeros(64)
-  d = seqops.ScanDesc()
+  d = seq_ref.ScanDesc()
   d.x = d.gate = d.h = d.last = buf.data_ptr() // 64 * 64
   d.T, d.N, d.D, d.G = 4, 2, 6, 3
   for k, v in kw.items():
@@ -217,7 +217,9 @@ def test_entry_points_refuse_before_any_launch():
   """Return code 1 and a reason, from arguments alone: none of these reaches a kernel."""
   import ctypes
 
-  lib = seqops._lib()
+  lib = native.lib()
+  assert lib.mjh_sizeof_scan_desc() == ctypes.sizeof(seq_ref.ScanDesc)
+  assert lib.mjh_sizeof_resnorm_desc() == ctypes.sizeof(seq_ref.ResnormDesc)
   bad = [(dict(T=0), b"positive"), (dict(D=0), b"positive"), (dict(G=4), b"divide"), (dict(dtype=7), b"type"),
          (dict(dtype=1, gtype=2), b"type"), (dict(mode=5), b"mode"), (dict(N=1 << 20, D=1 << 12, G=1), b"2^31"),
          (dict(h=None), b"needed")]
@@ -231,7 +233,7 @@ def test_entry_points_refuse_before_any_launch():
   assert lib.mjh_scan_backward(ctypes.byref(_scan_desc()), None) == 1
   assert lib.mjh_scan_step(ctypes.byref(_scan_desc()), None) == 1 and b"T must be 1" in lib.mjh_seq_last_error()
   assert lib.mjh_scan_workspace(ctypes.byref(_scan_desc(G=4)), 1) == -1
-  r = seqops.ResnormDesc()
+  r = seq_ref.ResnormDesc()
   r.R, r.D, r.pre = 2, 9000, 1
   for kw, why in ((dict(), b"8192"), (dict(D=8), b"residual is needed"), (dict(D=8, r=1024, gate=1024), b"need y"),
                   (dict(D=8, r=1024, n=None), b"output"), (dict(D=8, r=1024, n=1024, thr=1 << 33), b"threshold")):
@@ -246,6 +248,3 @@ def test_entry_points_refuse_before_any_launch():
   assert lib.mjh_dropout(None, 0, None, 0, 2, 2, 0, 1.0, 0, 0, 0, None, None, None) == 1
   assert lib.mjh_dropout(None, 0, None, 0, -1, 2, 0, 1.0, 0, 0, 0, None, None, None) == 1
   assert lib.mjh_dropout(None, 0, None, 0, 0, 2, 0, 1.0, 0, 0, 0, None, None, None) == 0
-  with pytest.raises(RuntimeError, match="mjh_x failed"):
-    seqops._check(1, "mjh_x")
-  assert native.CALLS["mjh_x"] == 1
