@@ -6,12 +6,13 @@
 //   n = norm_pre(s)
 // The statistics, s inside n, and all sums are float32; s and n are rounded once, at their store.
 //
-// A group of `TPR` lanes holds a row, 8 elements a lane, so every tensor is read once and every statistic is
-// taken from registers (the variance around the mean, in a second pass over registers). Groups up to a wave
-// reduce with lane exchanges, wider ones through shared memory. The backward pass keeps s and p nowhere: it
-// forms them again from y, residual and gate, the tensors that it has to read in any case, with the forward
-// pass's (mean, rstd) of each row. Weight gradients: a group adds its rows in registers, groups of a workgroup
-// join in shared memory, workgroups in a second launch, each in a fixed order.
+// A group of lanes holds a row, 8 elements a lane, so every tensor is read once and every statistic is taken from
+// registers (the variance around the mean, in a second pass over registers). Rows of up to 512 elements: 8 to 64
+// lanes, several rows a workgroup, sums by lane exchanges; longer rows: a workgroup of as many waves as they need,
+// sums joined in shared memory. The backward pass keeps s and p nowhere: it forms them again from y, residual and
+// gate, the tensors that it has to read in any case, with the forward pass's (mean, rstd) of each row. The next
+// row's loads are under way while a row is worked on. Weight gradients: a group adds its rows in registers, groups
+// of a workgroup join in shared memory, workgroups in a second launch, each in a fixed order.
 #include <algorithm>
 #include <cstring>
 
@@ -21,7 +22,8 @@ namespace {
 using namespace mjh_seq;
 
 constexpr int kPer = 8;     // elements a lane holds
-constexpr int kMaxTpr = 1024;
+constexpr int kMaxDim = 1024 * kPer;
+constexpr ll kColumnWaves = 256 * 4 * 4;  // waves of the wide rows' column stream: 4 a SIMD
 constexpr int kSums = 5;    // post weight, post bias, scale, pre weight, pre bias
 enum { kPostW, kPostB, kScale, kPreW, kPreB };
 
@@ -40,134 +42,189 @@ struct Args {
   void* dy; ll dys;
   void* dr; ll drs;
   void* dgate; ll dgs;
-  float* sums;    // (workgroups, kSums, D)
+  float* sums;    // (parts, kSums, D)
+  float* coef;    // (R, 4): the row sums of the wide rows' backward pass
   mjh_i64* ctr_out;
   Drop drop;
-  float eps;
+  float eps, inv;  // inv = 1 / D
   int R, D, layer, act, post, pre;
+  int tpr;    // lanes per row
+  int parts;  // workgroups (wide rows: row strands) of the backward pass
 };
 
-template <class T, bool VEC>
-struct Lanes {
-  static constexpr int kVec = VEC ? 16 / (int)sizeof(T) : 1;
-  static constexpr int kPieces = kPer / kVec;
-};
-// column of a lane's element k: pieces of kVec neighbours, a group's pieces side by side
-template <class T, bool VEC, int TPR>
-__device__ __forceinline__ int col(int lane, int k) {
-  constexpr int V = Lanes<T, VEC>::kVec;
-  return (k / V * TPR + lane) * V + k % V;
+// The sum over groups of L neighbouring lanes, in every lane: four steps inside a row of 16 lanes (neighbours, pairs,
+// then mirrored halves, whose lanes hold equal sums by then), the rest by lane exchange.
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
 }
-template <class T, bool VEC, int TPR>
-__device__ __forceinline__ void read(const T* p, int lane, int D, bool on, T (&o)[kPer]) {
-  constexpr int V = Lanes<T, VEC>::kVec;
-#pragma unroll
-  for (int k = 0; k < kPer; k += V) {
-    const int c = col<T, VEC, TPR>(lane, k);
-    Pack<T, V> v{};
-    if (on && c < D) v = load<T, V>(p + c);
-#pragma unroll
-    for (int j = 0; j < V; j++) o[k + j] = v.v[j];
-  }
-}
-template <class T, bool VEC, int TPR>
-__device__ __forceinline__ void write(T* p, int lane, int D, bool on, const float (&f)[kPer]) {
-  constexpr int V = Lanes<T, VEC>::kVec;
-#pragma unroll
-  for (int k = 0; k < kPer; k += V) {
-    const int c = col<T, VEC, TPR>(lane, k);
-    float o[V];
-#pragma unroll
-    for (int j = 0; j < V; j++) o[j] = f[k + j];
-    if (on && c < D) store<T, V>(p + c, o);
-  }
-}
-// channel weights; 1 or 0 where there are none
-template <class T, bool VEC, int TPR>
-__device__ __forceinline__ void weights(const void* w, int w32, int lane, int D, float none, float (&o)[kPer]) {
-#pragma unroll
-  for (int k = 0; k < kPer; k++) {
-    const int c = col<T, VEC, TPR>(lane, k);
-    o[k] = none;
-    if (w && c < D) o[k] = w32 ? static_cast<const float*>(w)[c] : (float)static_cast<const T*>(w)[c];
-  }
+template <int L>
+__device__ __forceinline__ float lane_sum(float v) {
+  v += dpp<0xB1>(v);                 // quad_perm 1 0 3 2
+  v += dpp<0x4E>(v);                 // quad_perm 2 3 0 1
+  v += dpp<0x141>(v);                // row_half_mirror
+  if (L >= 16) v += dpp<0x140>(v);   // row_mirror
+  if (L >= 32) v += __shfl_xor(v, 16);
+  if (L >= 64) v += __shfl_xor(v, 32);
+  return v;
 }
 
-// Sums of NV values over a row's lanes, in every lane. Wider groups than a wave: shared memory, two barriers.
-template <int TPR, int NV>
-__device__ __forceinline__ void row_sum(float (&v)[NV], float* shared) {
+// FULL: the row fills its lanes, so there is no column to check.
+
+constexpr int threads_of(int tpr) { return tpr > 64 ? tpr : 256; }
+
+// TPR: 8 to 64 lanes hold a row; above, the most threads of a workgroup that holds one (a.tpr of them do).
+template <class T, bool FULL, int TPR>
+struct Row {
+  static constexpr int kVec = 16 / (int)sizeof(T);
+  static constexpr bool kWide = TPR > 64;
+  static constexpr int kThreads = threads_of(TPR);
+  static constexpr int kGroups = kWide ? 1 : 256 / TPR;  // rows a workgroup holds
+  static constexpr int kWaves = kThreads / 64;
+  int lane, group, lanes, D;
+  __device__ __forceinline__ explicit Row(const Args& a) : D(a.D) {
+    lanes = kWide ? a.tpr : TPR;
+    lane = kWide ? threadIdx.x : threadIdx.x % TPR;
+    group = kWide ? 0 : threadIdx.x / TPR;
+  }
+  // column of the lane's element k: pieces of kVec neighbours, the lanes' pieces side by side
+  __device__ __forceinline__ int col(int k) const { return (k / kVec * lanes + lane) * kVec + k % kVec; }
+  __device__ __forceinline__ bool has(int k) const { return FULL || col(k) < D; }
+  // elements k .. k + N of a lane, which are neighbours; the row may end among them
+  template <class W, int N>
+  __device__ __forceinline__ Pack<W, N> piece(const W* q, int k) const {
+    Pack<W, N> v{};
+    if (FULL || col(k) + N <= D) {
+      v = load_loose<W, N>(q + col(k));
+    } else if (col(k) < D) {
 #pragma unroll
-  for (int m = (TPR < 64 ? TPR : 64) / 2; m > 0; m >>= 1)
-#pragma unroll
-    for (int k = 0; k < NV; k++) v[k] += __shfl_xor(v[k], m);
-  if constexpr (TPR > 64) {
-    constexpr int W = TPR / 64;
-    const int wave = threadIdx.x >> 6, first = wave / W * W;
-    if ((threadIdx.x & 63) == 0)
-#pragma unroll
-      for (int k = 0; k < NV; k++) shared[wave * NV + k] = v[k];
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < NV; k++) {
-      float t = 0.f;
-#pragma unroll
-      for (int j = 0; j < W; j++) t += shared[(first + j) * NV + k];
-      v[k] = t;
+      for (int j = 0; j < N; j++)
+        if (col(k + j) < D) v.v[j] = q[col(k + j)];
     }
-    __syncthreads();
+    return v;
   }
-}
-
-constexpr int block_of(int tpr) { return tpr < 256 ? 256 : tpr; }
-
-__device__ __forceinline__ unsigned long long drop_base(const Drop& d) { return mjh::Rng(d.seed, d.key, d.ctr).base; }
-
-// keep bits of a lane's elements (bit k: element k); the row's first element has index row * D
-template <class T, bool VEC, int TPR>
-__device__ __forceinline__ unsigned keep_bits(unsigned long long base, const Drop& d, ll first, int lane) {
-  constexpr int V = Lanes<T, VEC>::kVec;
-  unsigned bits = 0;
+  __device__ __forceinline__ void read(const void* p, ll row, ll step, bool on, T (&o)[kPer]) const {
+    const T* q = static_cast<const T*>(p) + row * step;
 #pragma unroll
-  for (int k = 0; k < kPer; k += V) {
-    const unsigned long long i = (unsigned long long)(first + col<T, VEC, TPR>(lane, k));
-    if (V > 1 && !(i & 1)) {
+    for (int k = 0; k < kPer; k += kVec) {
+      Pack<T, kVec> v{};
+      if (on) v = piece<T, kVec>(q, k);
 #pragma unroll
-      for (int j = 0; j < V; j += 2) {
-        const unsigned long long w = drop_word(base, (i + j) >> 1);
-        bits |= (unsigned)drop_keep(w, 0, d.thr) << (k + j);
-        bits |= (unsigned)drop_keep(w, 1, d.thr) << (k + j + 1);
+      for (int j = 0; j < kVec; j++) o[k + j] = v.v[j];
+    }
+  }
+  __device__ __forceinline__ void write(void* p, ll row, ll step, bool on, const float (&f)[kPer]) const {
+    if (!on) return;
+    T* q = static_cast<T*>(p) + row * step;
+#pragma unroll
+    for (int k = 0; k < kPer; k += kVec) {
+      float o[kVec];
+#pragma unroll
+      for (int j = 0; j < kVec; j++) o[j] = f[k + j];
+      if (FULL || col(k) + kVec <= D) {
+        store_loose<T, kVec>(q + col(k), o);
+      } else if (col(k) < D) {
+#pragma unroll
+        for (int j = 0; j < kVec; j++)
+          if (col(k + j) < D) q[col(k + j)] = (T)o[j];
       }
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; j++)
-        bits |= (unsigned)drop_keep(drop_word(base, (i + j) >> 1), (int)((i + j) & 1), d.thr) << (k + j);
     }
   }
-  return bits;
-}
-
-// mean and 1 / deviation of a row held in registers (columns beyond D hold 0 in v)
-template <class T, bool VEC, int TPR>
-__device__ __forceinline__ void row_stats(const float (&v)[kPer], const Args& a, int lane, float* shared, float& mean,
-                                          float& rstd) {
-  mean = 0.f;
-  float t[1];
-  if (a.layer) {
+  // channel weights; `none` where there are none
+  template <class W>
+  __device__ __forceinline__ void weights_as(const void* w, float (&o)[kPer]) const {
+    constexpr int kBy = kVec * (int)sizeof(W) > 16 ? 16 / (int)sizeof(W) : kVec;
+#pragma unroll
+    for (int k = 0; k < kPer; k += kBy) {
+      const auto v = piece<W, kBy>(static_cast<const W*>(w), k);
+#pragma unroll
+      for (int j = 0; j < kBy; j++)
+        if (has(k + j)) o[k + j] = (float)v.v[j];
+    }
+  }
+  __device__ __forceinline__ void weights(const void* w, int w32, float none, float (&o)[kPer]) const {
+#pragma unroll
+    for (int k = 0; k < kPer; k++) o[k] = none;
+    if (w) w32 ? weights_as<float>(w, o) : weights_as<T>(w, o);
+  }
+  __device__ __forceinline__ void scales(const Args& a, float (&o)[kPer]) const {
+    if (!a.scale_one) return weights(a.scale, a.w32, 1.f, o);
+    const float one = a.w32 ? *static_cast<const float*>(a.scale) : (float)*static_cast<const T*>(a.scale);
+#pragma unroll
+    for (int k = 0; k < kPer; k++) o[k] = one;
+  }
+  // Sums of NV values over a row's lanes, in every lane. Wide rows: shared memory (kWaves * NV floats), two barriers.
+  template <int NV>
+  __device__ __forceinline__ void sum(float (&v)[NV], float* shared) const {
+#pragma unroll
+    for (int k = 0; k < NV; k++) v[k] = lane_sum<(kWide ? 64 : TPR)>(v[k]);
+    if constexpr (kWide) {
+      const int wave = threadIdx.x >> 6, waves = lanes >> 6;
+      if ((threadIdx.x & 63) == 0)
+#pragma unroll
+        for (int k = 0; k < NV; k++) shared[wave * NV + k] = v[k];
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < NV; k++) v[k] = 0.f;
+#pragma unroll
+      for (int j = 0; j < kWaves; j++)
+        if (j < waves)
+#pragma unroll
+          for (int k = 0; k < NV; k++) v[k] += shared[j * NV + k];
+      __syncthreads();
+    }
+  }
+  // mean and 1 / deviation of a row held in registers (columns beyond D hold 0 in v)
+  __device__ __forceinline__ void stats(const float (&v)[kPer], const Args& a, float* shared, float& mean, float& rstd) const {
+    mean = 0.f;
+    float t[1];
+    if (a.layer) {
+      t[0] = 0.f;
+#pragma unroll
+      for (int k = 0; k < kPer; k++) t[0] += v[k];
+      sum<1>(t, shared);
+      mean = t[0] * a.inv;
+    }
     t[0] = 0.f;
 #pragma unroll
-    for (int k = 0; k < kPer; k++) t[0] += v[k];
-    row_sum<TPR, 1>(t, shared);
-    mean = t[0] / (float)a.D;
+    for (int k = 0; k < kPer; k++) {
+      const float c = has(k) ? v[k] - mean : 0.f;
+      t[0] += c * c;
+    }
+    sum<1>(t, shared);
+    rstd = __builtin_amdgcn_rsqf(__builtin_fmaf(t[0], a.inv, a.eps));  // to 1 ulp
   }
-  t[0] = 0.f;
+  // keep bits of the lane's elements (bit k: element k); the row's first element has index row * D. Neighbours
+  // share a word, and the words of a piece are one addition apart; in rows that begin at an odd index a piece
+  // begins with the second half of a word.
+  __device__ __forceinline__ unsigned keep_bits(unsigned long long base, const Drop& d, ll row) const {
+    unsigned bits = 0;
+    const bool odd = !FULL && (row * D & 1);
 #pragma unroll
-  for (int k = 0; k < kPer; k++) {
-    const float c = col<T, VEC, TPR>(lane, k) < a.D ? v[k] - mean : 0.f;
-    t[0] += c * c;
+    for (int k = 0; k < kPer; k += kVec) {
+      const unsigned long long i = (unsigned long long)(row * D + col(k));
+      unsigned long long z = base + ((i >> 1) + 1ull) * 0x9e3779b97f4a7c15ull, w = mjh::mix64(z);
+      if (odd) bits |= (unsigned)drop_keep(w, 1, d.thr) << k;
+#pragma unroll
+      for (int j = 0; j < kVec; j += 2) {
+        if (j > 0 || odd) {
+          z += 0x9e3779b97f4a7c15ull;
+          w = mjh::mix64(z);
+        }
+        const unsigned low = drop_keep(w, 0, d.thr), high = drop_keep(w, 1, d.thr);
+        if (odd) {
+          bits |= low << (k + j + 1);
+          if (j + 2 < kVec) bits |= high << (k + j + 2);
+        } else {
+          bits |= low << (k + j) | high << (k + j + 1);
+        }
+      }
+    }
+    return bits;
   }
-  row_sum<TPR, 1>(t, shared);
-  rstd = 1.f / sqrtf(t[0] / (float)a.D + a.eps);
-}
+};
+
+__device__ __forceinline__ unsigned long long drop_base(const Drop& d) { return mjh::Rng(d.seed, d.key, d.ctr).base; }
 
 struct Act {
   float value, slope;
@@ -187,169 +244,235 @@ struct Act {
   }
 };
 
-template <class T, bool VEC, int TPR>
-__global__ __launch_bounds__(block_of(TPR)) void resnorm_forward(const Args a) {
-  constexpr int kGroups = block_of(TPR) / TPR;
-  __shared__ float shared[block_of(TPR) / 64];
-  const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
+// act(gate) (and its slope) of a lane's elements; one branch for all
+template <class T, bool SLOPE, int N>
+__device__ __forceinline__ void activate(const T (&g)[N], const Args& a, float (&value)[N], float (&slope)[N]) {
+  if (!a.gate) {
+#pragma unroll
+    for (int k = 0; k < N; k++) value[k] = 1.f, slope[k] = 0.f;
+  } else if (a.act == MJH_ACT_SIGMOID) {
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+      const Act t((float)g[k], MJH_ACT_SIGMOID);
+      value[k] = t.value;
+      if (SLOPE) slope[k] = t.slope;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+      const Act t((float)g[k], MJH_ACT_SILU);
+      value[k] = t.value;
+      if (SLOPE) slope[k] = t.slope;
+    }
+  }
+}
+
+template <class T, bool FULL, int TPR>
+__global__ __launch_bounds__(threads_of(TPR)) void resnorm_forward(const Args a) {
+  typedef Row<T, FULL, TPR> R;
+  __shared__ float shared[R::kWaves];
+  const R at(a);
   if (a.ctr_out && blockIdx.x == 0 && threadIdx.x == 0) *a.ctr_out = a.drop.ctr ? *a.drop.ctr : 0;
   const bool block = a.y != nullptr;
   const unsigned long long base = a.drop.thr ? drop_base(a.drop) : 0;
+  // A workgroup of more than 256 threads takes the weights from the cache at every row and loads no row ahead: the
+  // registers buy a second workgroup on the CU instead.
+  constexpr bool kHold = R::kThreads <= 256;
   float post_w[kPer], post_b[kPer], pre_w[kPer], pre_b[kPer], scale[kPer];
-  weights<T, VEC, TPR>(a.post_w, a.w32, lane, a.D, 1.f, post_w);
-  weights<T, VEC, TPR>(a.post_b, a.w32, lane, a.D, 0.f, post_b);
-  weights<T, VEC, TPR>(a.pre_w, a.w32, lane, a.D, 1.f, pre_w);
-  weights<T, VEC, TPR>(a.pre_b, a.w32, lane, a.D, 0.f, pre_b);
-  weights<T, VEC, TPR>(a.scale_one ? nullptr : a.scale, a.w32, lane, a.D, 1.f, scale);
-  if (a.scale_one) {
-    const float one = a.w32 ? *static_cast<const float*>(a.scale) : (float)*static_cast<const T*>(a.scale);
-#pragma unroll
-    for (int k = 0; k < kPer; k++) scale[k] = one;
+  if (kHold) {
+    at.weights(a.post_w, a.w32, 1.f, post_w);
+    at.weights(a.post_b, a.w32, 0.f, post_b);
+    at.weights(a.pre_w, a.w32, 1.f, pre_w);
+    at.weights(a.pre_b, a.w32, 0.f, pre_b);
+    at.scales(a, scale);
   }
-  for (ll first = (ll)blockIdx.x * kGroups; first < a.R; first += (ll)gridDim.x * kGroups) {
-    const ll row = first + group;
+  struct {
+    T r[kPer], y[kPer], g[kPer];
+  } cur, next;
+  auto fetch = [&](auto& to, ll row) {
     const bool on = row < a.R;
-    T rr[kPer];
-    read<T, VEC, TPR>(static_cast<const T*>(a.r) + row * a.rs, lane, a.D, on, rr);
+    at.read(a.r, row, a.rs, on, to.r);
+    if (block) at.read(a.y, row, a.ys, on, to.y);
+    if (a.gate) at.read(a.gate, row, a.gs, on, to.g);
+  };
+  const ll step = (ll)gridDim.x * R::kGroups;
+  fetch(cur, (ll)blockIdx.x * R::kGroups + at.group);
+  for (ll first = (ll)blockIdx.x * R::kGroups; first < a.R; first += step) {
+    const ll row = first + at.group;
+    const bool on = row < a.R;
+    if (kHold) fetch(next, row + step);
     float s[kPer], stats[4] = {0.f, 1.f, 0.f, 1.f};
+#pragma unroll
+    for (int k = 0; k < kPer; k++) s[k] = (float)cur.r[k];
     if (block) {
-      T ry[kPer], rg[kPer];
-      read<T, VEC, TPR>(static_cast<const T*>(a.y) + row * a.ys, lane, a.D, on, ry);
-      if (a.gate) read<T, VEC, TPR>(static_cast<const T*>(a.gate) + row * a.gs, lane, a.D, on, rg);
-      float y[kPer];
+      float p[kPer], av[kPer], slope[kPer];
 #pragma unroll
-      for (int k = 0; k < kPer; k++) y[k] = (float)ry[k];
-      if (a.post) row_stats<T, VEC, TPR>(y, a, lane, shared, stats[0], stats[1]);
-      const unsigned keep = a.drop.thr ? keep_bits<T, VEC, TPR>(base, a.drop, row * a.D, lane) : ~0u;
+      for (int k = 0; k < kPer; k++) p[k] = (float)cur.y[k];
+      if (a.post) {
+        at.stats(p, a, shared, stats[0], stats[1]);
+        if (!kHold) {
+          at.weights(a.post_w, a.w32, 1.f, post_w);
+          at.weights(a.post_b, a.w32, 0.f, post_b);
+        }
 #pragma unroll
-      for (int k = 0; k < kPer; k++) {
-        float p = a.post ? (y[k] - stats[0]) * stats[1] * post_w[k] + post_b[k] : y[k];
-        p = (keep >> k & 1u) ? p * a.drop.scale : 0.f;
-        if (a.gate) p *= Act((float)rg[k], a.act).value;
-        s[k] = (float)rr[k] + scale[k] * p;
+        for (int k = 0; k < kPer; k++) p[k] = __builtin_fmaf((p[k] - stats[0]) * stats[1], post_w[k], post_b[k]);
       }
-      write<T, VEC, TPR>(static_cast<T*>(a.s) + row * a.ss, lane, a.D, on, s);
-    } else {
+      if (a.drop.thr) {
+        const unsigned keep = at.keep_bits(base, a.drop, row);
 #pragma unroll
-      for (int k = 0; k < kPer; k++) s[k] = (float)rr[k];
+        for (int k = 0; k < kPer; k++) p[k] = (keep >> k & 1u) ? p[k] * a.drop.scale : 0.f;
+      }
+      activate<T, false>(cur.g, a, av, slope);
+      if (!kHold) at.scales(a, scale);
+#pragma unroll
+      for (int k = 0; k < kPer; k++) s[k] = __builtin_fmaf(scale[k], av[k] * p[k], s[k]);
+      at.write(a.s, row, a.ss, on, s);
     }
     if (a.pre) {
 #pragma unroll
       for (int k = 0; k < kPer; k++)
-        if (col<T, VEC, TPR>(lane, k) >= a.D) s[k] = 0.f;
-      row_stats<T, VEC, TPR>(s, a, lane, shared, stats[2], stats[3]);
-      float n[kPer];
+        if (!at.has(k)) s[k] = 0.f;
+      at.stats(s, a, shared, stats[2], stats[3]);
+      if (!kHold) {
+        at.weights(a.pre_w, a.w32, 1.f, pre_w);
+        at.weights(a.pre_b, a.w32, 0.f, pre_b);
+      }
 #pragma unroll
-      for (int k = 0; k < kPer; k++) n[k] = (s[k] - stats[2]) * stats[3] * pre_w[k] + pre_b[k];
-      write<T, VEC, TPR>(static_cast<T*>(a.n) + row * a.ns, lane, a.D, on, n);
+      for (int k = 0; k < kPer; k++) s[k] = __builtin_fmaf((s[k] - stats[2]) * stats[3], pre_w[k], pre_b[k]);
+      at.write(a.n, row, a.ns, on, s);
     }
-    if (a.stats && on && lane == 0) store<float, 4>(a.stats + row * 4, stats);
+    if (a.stats && on && at.lane == 0) store<float, 4>(a.stats + row * 4, stats);
+    if (kHold)
+      cur = next;
+    else
+      fetch(cur, row + step);
   }
 }
 
-// BLOCK: there is a y (else only the norm before). BIAS: bias gradients are wanted.
-template <class T, bool VEC, int TPR, bool BLOCK, bool BIAS>
-__global__ __launch_bounds__(block_of(TPR)) void resnorm_backward(const Args a) {
-  constexpr int kGroups = block_of(TPR) / TPR;
-  __shared__ float shared[block_of(TPR) / 64 * 2];
-  __shared__ float join[kGroups > 1 ? block_of(TPR) * kPer : 1];
-  const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
+// BLOCK: there is a y (else only the norm before). BIAS: there are biases.
+template <class T, bool FULL, int TPR, bool BLOCK, bool BIAS>
+__global__ __launch_bounds__(threads_of(TPR)) void resnorm_backward(const Args a) {
+  typedef Row<T, FULL, TPR> R;
+  __shared__ float shared[R::kWaves * 2];
+  __shared__ float join[R::kGroups > 1 ? 256 * kPer : 1];
+  const R at(a);
   const unsigned long long base = BLOCK && a.drop.thr ? drop_base(a.drop) : 0;
   float post_w[kPer], post_b[kPer], pre_w[kPer], scale[kPer];
-  weights<T, VEC, TPR>(a.pre_w, a.w32, lane, a.D, 1.f, pre_w);
+  at.weights(a.pre_w, a.w32, 1.f, pre_w);
   if (BLOCK) {
-    weights<T, VEC, TPR>(a.post_w, a.w32, lane, a.D, 1.f, post_w);
-    weights<T, VEC, TPR>(BIAS ? a.post_b : nullptr, a.w32, lane, a.D, 0.f, post_b);
-    weights<T, VEC, TPR>(a.scale_one ? nullptr : a.scale, a.w32, lane, a.D, 1.f, scale);
-    if (a.scale_one) {
-      const float one = a.w32 ? *static_cast<const float*>(a.scale) : (float)*static_cast<const T*>(a.scale);
-#pragma unroll
-      for (int k = 0; k < kPer; k++) scale[k] = one;
-    }
+    at.weights(a.post_w, a.w32, 1.f, post_w);
+    if (BIAS) at.weights(a.post_b, a.w32, 0.f, post_b);
+    at.scales(a, scale);
   }
   float sum[kSums][kPer];
 #pragma unroll
   for (int q = 0; q < kSums; q++)
 #pragma unroll
     for (int k = 0; k < kPer; k++) sum[q][k] = 0.f;
-  const float inv = 1.f / (float)a.D;
-  for (ll first = (ll)blockIdx.x * kGroups; first < a.R; first += (ll)gridDim.x * kGroups) {
-    const ll row = first + group;
+  struct {
+    T r[kPer], y[kPer], g[kPer], ds[kPer], dn[kPer];
+    Pack<float, 4> st;
+  } cur, next;
+  auto fetch = [&](auto& to, ll row) {
     const bool on = row < a.R;
-    T rr[kPer], ry[kPer], rg[kPer], rds[kPer], rdn[kPer];
-    if (a.pre) read<T, VEC, TPR>(static_cast<const T*>(a.r) + row * a.rs, lane, a.D, on, rr);
+    to.st = Pack<float, 4>{};
+    if (on) to.st = load<float, 4>(a.stats + row * 4);
     if (BLOCK) {
-      read<T, VEC, TPR>(static_cast<const T*>(a.y) + row * a.ys, lane, a.D, on, ry);
-      if (a.gate) read<T, VEC, TPR>(static_cast<const T*>(a.gate) + row * a.gs, lane, a.D, on, rg);
+      at.read(a.y, row, a.ys, on, to.y);
+      if (a.gate) at.read(a.gate, row, a.gs, on, to.g);
     }
-    if (a.ds) read<T, VEC, TPR>(static_cast<const T*>(a.ds) + row * a.dss, lane, a.D, on, rds);
-    if (a.dn) read<T, VEC, TPR>(static_cast<const T*>(a.dn) + row * a.dns, lane, a.D, on, rdn);
-    Pack<float, 4> st{};
-    if (on) st = load<float, 4>(a.stats + row * 4);
-    const unsigned keep = BLOCK && a.drop.thr ? keep_bits<T, VEC, TPR>(base, a.drop, row * a.D, lane) : ~0u;
-    float ds[kPer], yhat[kPer], u[kPer], av[kPer], slope[kPer];
+    if (a.dn) {
+      at.read(a.r, row, a.rs, on, to.r);
+      at.read(a.dn, row, a.dns, on, to.dn);
+    }
+    if (a.ds) at.read(a.ds, row, a.dss, on, to.ds);
+  };
+  const ll step = (ll)gridDim.x * R::kGroups;
+  fetch(cur, (ll)blockIdx.x * R::kGroups + at.group);
+  for (ll first = (ll)blockIdx.x * R::kGroups; first < a.R; first += step) {
+    const ll row = first + at.group;
+    const bool on = row < a.R;
+    fetch(next, row + step);
+    const float mean = cur.st.v[0], rstd = cur.st.v[1], pre_mean = cur.st.v[2], pre_rstd = cur.st.v[3];
+    bool in[kPer];
 #pragma unroll
-    for (int k = 0; k < kPer; k++) {
-      ds[k] = a.ds ? (float)rds[k] : 0.f;
-      if (BLOCK) {
-        yhat[k] = a.post ? ((float)ry[k] - st.v[0]) * st.v[1] : (float)ry[k];
-        const float p = a.post ? yhat[k] * post_w[k] + post_b[k] : yhat[k];
-        u[k] = (keep >> k & 1u) ? p * a.drop.scale : 0.f;
-        av[k] = 1.f;
-        slope[k] = 0.f;
-        if (a.gate) {
-          const Act t((float)rg[k], a.act);
-          av[k] = t.value;
-          slope[k] = t.slope;
+    for (int k = 0; k < kPer; k++) in[k] = on && at.has(k);
+    float ds[kPer], yhat[kPer], u[kPer], av[kPer], slope[kPer];
+    unsigned keep = ~0u;
+#pragma unroll
+    for (int k = 0; k < kPer; k++) ds[k] = 0.f;
+    if (a.ds) {
+#pragma unroll
+      for (int k = 0; k < kPer; k++) ds[k] = (float)cur.ds[k];
+    }
+    if (BLOCK) {
+#pragma unroll
+      for (int k = 0; k < kPer; k++) u[k] = yhat[k] = (float)cur.y[k];
+      if (a.post) {
+#pragma unroll
+        for (int k = 0; k < kPer; k++) {
+          yhat[k] = (yhat[k] - mean) * rstd;
+          u[k] = BIAS ? __builtin_fmaf(yhat[k], post_w[k], post_b[k]) : yhat[k] * post_w[k];
         }
       }
+      if (a.drop.thr) {
+        keep = at.keep_bits(base, a.drop, row);
+#pragma unroll
+        for (int k = 0; k < kPer; k++) u[k] = (keep >> k & 1u) ? u[k] * a.drop.scale : 0.f;
+      }
+      activate<T, true>(cur.g, a, av, slope);
     }
     if (a.dn) {
       float hat[kPer], t[2] = {0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < kPer; k++) {
-        const bool in = on && col<T, VEC, TPR>(lane, k) < a.D;
-        const float s = BLOCK ? (float)rr[k] + scale[k] * (av[k] * u[k]) : (float)rr[k];
-        hat[k] = in ? (s - st.v[2]) * st.v[3] : 0.f;
-        const float dn = (float)rdn[k];
+        const float r = (float)cur.r[k];
+        const float s = BLOCK ? __builtin_fmaf(scale[k], av[k] * u[k], r) : r;
+        hat[k] = in[k] ? (s - pre_mean) * pre_rstd : 0.f;
+        const float dn = (float)cur.dn[k];
         sum[kPreW][k] += dn * hat[k];
         if (BIAS) sum[kPreB][k] += dn;
-        const float dv = in ? dn * pre_w[k] : 0.f;
+        const float dv = in[k] ? dn * pre_w[k] : 0.f;
         t[0] += dv * hat[k];
         t[1] += dv;
       }
-      row_sum<TPR, 2>(t, shared);
-      const float c0 = t[0] * inv, c1 = a.layer ? t[1] * inv : 0.f;
+      at.template sum<2>(t, shared);
+      const float c0 = t[0] * a.inv, c1 = a.layer ? t[1] * a.inv : 0.f;
 #pragma unroll
-      for (int k = 0; k < kPer; k++) ds[k] += ((float)rdn[k] * pre_w[k] - hat[k] * c0 - c1) * st.v[3];
+      for (int k = 0; k < kPer; k++) ds[k] += ((float)cur.dn[k] * pre_w[k] - hat[k] * c0 - c1) * pre_rstd;
     }
-    if (a.dr) write<T, VEC, TPR>(static_cast<T*>(a.dr) + row * a.drs, lane, a.D, on, ds);
+    if (a.dr) at.write(a.dr, row, a.drs, on, ds);
     if (BLOCK) {
-      float dp[kPer], dg[kPer], t[2] = {0.f, 0.f};
+      float dg[kPer], t[2] = {0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < kPer; k++) {
-        const bool in = on && col<T, VEC, TPR>(lane, k) < a.D;
-        if (in) sum[kScale][k] += ds[k] * (av[k] * u[k]);
+        if (in[k]) sum[kScale][k] += ds[k] * (av[k] * u[k]);
         const float dw = ds[k] * scale[k];
         dg[k] = dw * u[k] * slope[k];
-        dp[k] = in && (keep >> k & 1u) ? dw * av[k] * a.drop.scale : 0.f;
-        if (a.post) {
-          if (in) sum[kPostW][k] += dp[k] * yhat[k];
-          if (BIAS) sum[kPostB][k] += dp[k];
-          dp[k] *= post_w[k];
-          if (in) t[0] += dp[k] * yhat[k];
-          t[1] += dp[k];
-        }
+        ds[k] = in[k] ? dw * av[k] : 0.f;
       }
-      if (a.gate && a.dgate) write<T, VEC, TPR>(static_cast<T*>(a.dgate) + row * a.dgs, lane, a.D, on, dg);
-      if (a.post) {
-        row_sum<TPR, 2>(t, shared);
-        const float c0 = t[0] * inv, c1 = a.layer ? t[1] * inv : 0.f;
+      if (a.drop.thr) {
 #pragma unroll
-        for (int k = 0; k < kPer; k++) dp[k] = (dp[k] - yhat[k] * c0 - c1) * st.v[1];
+        for (int k = 0; k < kPer; k++) ds[k] = (keep >> k & 1u) ? ds[k] * a.drop.scale : 0.f;
       }
-      if (a.dy) write<T, VEC, TPR>(static_cast<T*>(a.dy) + row * a.dys, lane, a.D, on, dp);
+      if (a.gate && a.dgate) at.write(a.dgate, row, a.dgs, on, dg);
+      if (a.post) {
+#pragma unroll
+        for (int k = 0; k < kPer; k++) {
+          if (in[k]) sum[kPostW][k] += ds[k] * yhat[k];
+          if (BIAS) sum[kPostB][k] += ds[k];
+          ds[k] *= post_w[k];
+          if (in[k]) t[0] += ds[k] * yhat[k];
+          t[1] += ds[k];
+        }
+        at.template sum<2>(t, shared);
+        const float c0 = t[0] * a.inv, c1 = a.layer ? t[1] * a.inv : 0.f;
+#pragma unroll
+        for (int k = 0; k < kPer; k++) ds[k] = (ds[k] - yhat[k] * c0 - c1) * rstd;
+      }
+      if (a.dy) at.write(a.dy, row, a.dys, on, ds);
     }
+    cur = next;
   }
   if (!a.sums) return;
   float* out = a.sums + (ll)blockIdx.x * kSums * a.D;
@@ -357,51 +480,308 @@ __global__ __launch_bounds__(block_of(TPR)) void resnorm_backward(const Args a) 
   for (int q = 0; q < kSums; q++) {
     if (!BLOCK && q < kPreW) continue;
     if (!BIAS && (q == kPostB || q == kPreB)) continue;
-    if constexpr (kGroups > 1) {
+    if constexpr (R::kGroups > 1) {
       __syncthreads();
 #pragma unroll
-      for (int k = 0; k < kPer; k++) join[k * block_of(TPR) + threadIdx.x] = sum[q][k];
+      for (int k = 0; k < kPer; k++) join[k * 256 + threadIdx.x] = sum[q][k];
       __syncthreads();
-      if (group == 0)
+      if (at.group == 0)
 #pragma unroll
         for (int k = 0; k < kPer; k++) {
           float t = 0.f;
-          for (int g = 0; g < kGroups; g++) t += join[k * block_of(TPR) + g * TPR + lane];
+          for (int g = 0; g < R::kGroups; g++) t += join[k * 256 + g * TPR + at.lane];
           sum[q][k] = t;
         }
     }
-    if (group == 0)
+    if (at.group == 0)
 #pragma unroll
-      for (int k = 0; k < kPer; k++) {
-        const int c = col<T, VEC, TPR>(lane, k);
-        if (c < a.D) out[q * a.D + c] = sum[q][k];
+      for (int k = 0; k < kPer; k++)
+        if (at.has(k)) out[q * a.D + at.col(k)] = sum[q][k];
+  }
+}
+
+// ---- backward of rows longer than 2,048 elements ----
+// Held in registers, such a row with its weight sums leaves one workgroup a CU and nothing to hide its barriers
+// (2,047 x 4,097 floats: 170 us). Instead two streams: the first takes a row's sums, the second, whose threads own
+// columns and walk the rows, forms the gradients and the columns' sums. It reads the inputs again, largely from the
+// cache behind the L2.
+//
+// The norm of y needs sums over ds, the gradient of s, which itself has the row's sums c0, c1 in it. It is linear
+// in them, ds = X - rstd (hat c0 + c1) with X = ds_in + rstd dn w, so the first stream takes the sums of X q, hat q
+// and q (q = the factor from ds to the gradient of the normalised y, once times yhat, once alone) in the same pass.
+template <class T>
+struct Piece {
+  static constexpr int N = 16 / (int)sizeof(T);
+  int c, D;
+  template <class W, int M>
+  __device__ __forceinline__ Pack<W, M> get(const W* q, int at) const {
+    Pack<W, M> v{};
+    if (at + M <= D) {
+      v = load_loose<W, M>(q + at);
+    } else if (at < D) {
+#pragma unroll
+      for (int j = 0; j < M; j++)
+        if (at + j < D) v.v[j] = q[at + j];
+    }
+    return v;
+  }
+  __device__ __forceinline__ Pack<T, N> read(const void* p, ll row, ll step) const {
+    return get<T, N>(static_cast<const T*>(p) + row * step, c);
+  }
+  __device__ __forceinline__ void write(void* p, ll row, ll step, const float (&f)[N]) const {
+    T* q = static_cast<T*>(p) + row * step + c;
+    if (c + N <= D) {
+      store_loose<T, N>(q, f);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; j++)
+        if (c + j < D) q[j] = (T)f[j];
+    }
+  }
+  __device__ __forceinline__ void weights(const void* w, int w32, float none, float (&o)[N]) const {
+#pragma unroll
+    for (int j = 0; j < N; j++) o[j] = none;
+    if (!w) return;
+    if (w32) {
+#pragma unroll
+      for (int k = 0; k < N; k += 4) {
+        const auto v = get<float, 4>(static_cast<const float*>(w), c + k);
+#pragma unroll
+        for (int j = 0; j < 4; j++) o[k + j] = v.v[j];
       }
+    } else {
+      const auto v = get<T, N>(static_cast<const T*>(w), c);
+#pragma unroll
+      for (int j = 0; j < N; j++) o[j] = (float)v.v[j];
+    }
+  }
+  __device__ __forceinline__ void scales(const Args& a, float (&o)[N]) const {
+    if (!a.scale_one) return weights(a.scale, a.w32, 1.f, o);
+    const float one = a.w32 ? *static_cast<const float*>(a.scale) : (float)*static_cast<const T*>(a.scale);
+#pragma unroll
+    for (int j = 0; j < N; j++) o[j] = one;
+  }
+  __device__ __forceinline__ unsigned keep_bits(unsigned long long base, const Drop& d, ll row) const {
+    unsigned bits = 0;
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+      const unsigned long long i = (unsigned long long)(row * D + c + j);
+      bits |= (unsigned)drop_keep(drop_word(base, i >> 1), (int)(i & 1), d.thr) << j;
+    }
+    return bits;
+  }
+};
+
+// What both streams form of a row's piece before its sums are known.
+template <class T, bool BLOCK, bool BIAS>
+struct Formed {
+  static constexpr int N = Piece<T>::N;
+  float ds[N], dn[N], hat[N], yhat[N], u[N], av[N], slope[N];
+  unsigned keep;
+  template <class Raw>
+  __device__ __forceinline__ Formed(const Args& a, const Piece<T>& at, const Raw& raw, const Pack<float, 4>& st, ll row,
+                                    unsigned long long base, const float (&post_w)[N], const float (&post_b)[N],
+                                    const float (&scale)[N]) {
+    keep = ~0u;
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+      ds[j] = a.ds ? (float)raw.ds.v[j] : 0.f;
+      dn[j] = a.dn ? (float)raw.dn.v[j] : 0.f;
+      hat[j] = a.dn ? (float)raw.r.v[j] : 0.f;
+    }
+    if (BLOCK) {
+#pragma unroll
+      for (int j = 0; j < N; j++) {
+        yhat[j] = (float)raw.y.v[j];
+        if (a.post) yhat[j] = (yhat[j] - st.v[0]) * st.v[1];
+        u[j] = a.post ? (BIAS ? __builtin_fmaf(yhat[j], post_w[j], post_b[j]) : yhat[j] * post_w[j]) : yhat[j];
+      }
+      if (a.drop.thr) {
+        keep = at.keep_bits(base, a.drop, row);
+#pragma unroll
+        for (int j = 0; j < N; j++) u[j] = (keep >> j & 1u) ? u[j] * a.drop.scale : 0.f;
+      }
+      activate<T, true>(raw.g.v, a, av, slope);
+    }
+    if (a.dn) {
+#pragma unroll
+      for (int j = 0; j < N; j++) {
+        const float s = BLOCK ? __builtin_fmaf(scale[j], av[j] * u[j], hat[j]) : hat[j];
+        hat[j] = at.c + j < a.D ? (s - st.v[2]) * st.v[3] : 0.f;
+      }
+    }
+  }
+};
+template <class T>
+struct Raw {
+  Pack<T, Piece<T>::N> y, r, g, ds, dn;
+  template <bool BLOCK>
+  __device__ __forceinline__ void fetch(const Args& a, const Piece<T>& at, ll row) {
+    if (BLOCK) {
+      y = at.read(a.y, row, a.ys);
+      if (a.gate) g = at.read(a.gate, row, a.gs);
+    }
+    if (a.dn) {
+      r = at.read(a.r, row, a.rs);
+      dn = at.read(a.dn, row, a.dns);
+    }
+    if (a.ds) ds = at.read(a.ds, row, a.dss);
+  }
+};
+
+// One workgroup a row: (c0, c1) of the norm before, (c0, c1) of the norm of y.
+template <class T, bool BLOCK, bool BIAS>
+__global__ __launch_bounds__(256) void resnorm_rows(const Args a) {
+  constexpr int N = Piece<T>::N;
+  __shared__ float shared[4][8];
+  const ll row = blockIdx.x;
+  const unsigned long long base = BLOCK && a.drop.thr ? drop_base(a.drop) : 0;
+  const auto st = load<float, 4>(a.stats + row * 4);
+  float t[8] = {};  // dv hat, dv, X q0, hat q0, q0, X q1, hat q1, q1
+  for (int c = threadIdx.x * N; c < a.D; c += 256 * N) {
+    const Piece<T> at{c, a.D};
+    Raw<T> raw;
+    raw.template fetch<BLOCK>(a, at, row);
+    float pre_w[N], post_w[N], post_b[N], scale[N];
+    at.weights(a.pre_w, a.w32, 1.f, pre_w);
+    if (BLOCK) {
+      at.weights(a.post_w, a.w32, 1.f, post_w);
+      if (BIAS) at.weights(a.post_b, a.w32, 0.f, post_b);
+      at.scales(a, scale);
+    }
+    const Formed<T, BLOCK, BIAS> f(a, at, raw, st, row, base, post_w, post_b, scale);
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+      if (c + j >= a.D) continue;
+      const float dv = f.dn[j] * pre_w[j];
+      t[0] += dv * f.hat[j];
+      t[1] += dv;
+      if (BLOCK) {
+        const float x = __builtin_fmaf(dv, st.v[3], f.ds[j]);
+        float q = scale[j] * f.av[j] * post_w[j];
+        q = (f.keep >> j & 1u) ? (a.drop.thr ? q * a.drop.scale : q) : 0.f;
+        const float q0 = q * f.yhat[j];
+        t[2] += x * q0;
+        t[3] += f.hat[j] * q0;
+        t[4] += q0;
+        t[5] += x * q;
+        t[6] += f.hat[j] * q;
+        t[7] += q;
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 8; k++) {
+    t[k] = lane_sum<64>(t[k]);
+    if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6][k] = t[k];
+  }
+  __syncthreads();
+  if (threadIdx.x) return;
+#pragma unroll
+  for (int k = 0; k < 8; k++) t[k] = ((shared[0][k] + shared[1][k]) + (shared[2][k] + shared[3][k])) * a.inv;
+  const float c0 = t[0], c1 = a.layer ? t[1] : 0.f;
+  const float out[4] = {c0, c1, t[2] - st.v[3] * (c0 * t[3] + c1 * t[4]),
+                        a.layer ? t[5] - st.v[3] * (c0 * t[6] + c1 * t[7]) : 0.f};
+  store<float, 4>(a.coef + row * 4, out);
+}
+
+// A wave owns 64 pieces of columns and walks rows blockIdx.y, + gridDim.y, ...
+template <class T, bool BLOCK, bool BIAS>
+__global__ __launch_bounds__(64) void resnorm_columns(const Args a) {
+  constexpr int N = Piece<T>::N;
+  const Piece<T> at{(int)(blockIdx.x * 64 + threadIdx.x) * N, a.D};
+  if (at.c >= a.D) return;
+  const unsigned long long base = BLOCK && a.drop.thr ? drop_base(a.drop) : 0;
+  float pre_w[N], post_w[N], post_b[N], scale[N];
+  at.weights(a.pre_w, a.w32, 1.f, pre_w);
+  if (BLOCK) {
+    at.weights(a.post_w, a.w32, 1.f, post_w);
+    if (BIAS) at.weights(a.post_b, a.w32, 0.f, post_b);
+    at.scales(a, scale);
+  }
+  float sum[kSums][N];
+#pragma unroll
+  for (int q = 0; q < kSums; q++)
+#pragma unroll
+    for (int j = 0; j < N; j++) sum[q][j] = 0.f;
+  Raw<T> cur, next;
+  cur.template fetch<BLOCK>(a, at, blockIdx.y);
+  for (ll row = blockIdx.y; row < a.R; row += gridDim.y) {
+    if (row + gridDim.y < a.R) next.template fetch<BLOCK>(a, at, row + gridDim.y);
+    const auto st = load<float, 4>(a.stats + row * 4), k = load<float, 4>(a.coef + row * 4);
+    const Formed<T, BLOCK, BIAS> f(a, at, cur, st, row, base, post_w, post_b, scale);
+    float ds[N], dg[N];
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+      ds[j] = f.ds[j];
+      if (a.dn) {
+        ds[j] += (f.dn[j] * pre_w[j] - f.hat[j] * k.v[0] - k.v[1]) * st.v[3];
+        sum[kPreW][j] += f.dn[j] * f.hat[j];
+        if (BIAS) sum[kPreB][j] += f.dn[j];
+      }
+    }
+    if (a.dr) at.write(a.dr, row, a.drs, ds);
+    if (BLOCK) {
+#pragma unroll
+      for (int j = 0; j < N; j++) {
+        sum[kScale][j] += ds[j] * (f.av[j] * f.u[j]);
+        const float dw = ds[j] * scale[j];
+        dg[j] = dw * f.u[j] * f.slope[j];
+        ds[j] = (f.keep >> j & 1u) ? (a.drop.thr ? dw * f.av[j] * a.drop.scale : dw * f.av[j]) : 0.f;
+        if (a.post) {
+          sum[kPostW][j] += ds[j] * f.yhat[j];
+          if (BIAS) sum[kPostB][j] += ds[j];
+          ds[j] = (ds[j] * post_w[j] - f.yhat[j] * k.v[2] - k.v[3]) * st.v[1];
+        }
+      }
+      if (a.gate && a.dgate) at.write(a.dgate, row, a.dgs, dg);
+      if (a.dy) at.write(a.dy, row, a.dys, ds);
+    }
+    cur = next;
+  }
+  if (!a.sums) return;
+  float* out = a.sums + (ll)blockIdx.y * kSums * a.D;
+#pragma unroll
+  for (int q = 0; q < kSums; q++) {
+    if (!BLOCK && q < kPreW) continue;
+    if (!BIAS && (q == kPostB || q == kPreB)) continue;
+#pragma unroll
+    for (int j = 0; j < N; j++)
+      if (at.c + j < a.D) out[q * a.D + at.c + j] = sum[q][j];
   }
 }
 
 struct Join {
-  const float* sums; int parts, D, rows32;  // rows32: outputs are float32 (else T)
+  const float* sums;
+  int parts, D, w32;  // w32: outputs are float32 (else T)
+  int q[kSums];       // the sums that are wanted
   void* out[kSums];
-  int scale_one;
-  float* scale_cols;  // the scale's column sums where one scale serves all columns
+  float* scale_cols;  // the scale's column sums where one scale serves all columns (else NULL)
 };
 
-// Column sums of the workgroups' partial sums: 64 columns by 4 strands of workgroups, joined in their order.
+// Column sums of the workgroups' partial sums: 32 columns by 32 strands of workgroups, loads of a strand
+// independent of each other (64 columns by 4 strands took 62 us for 1,024 workgroups, this 5); strands joined in
+// their order.
 template <class T>
-__global__ __launch_bounds__(256) void resnorm_join(const Join j) {
-  __shared__ float strand[4][64];
-  const int q = blockIdx.y, c = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
-  if (!j.out[q]) return;
+__global__ __launch_bounds__(1024) void resnorm_join(const Join j) {
+  __shared__ float strand[32][33];
+  const int q = j.q[blockIdx.y], x = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + x;
   float t = 0.f;
-  if (c < j.D)
-    for (int p = w; p < j.parts; p += 4) t += j.sums[((ll)p * kSums + q) * j.D + c];
-  strand[w][threadIdx.x & 63] = t;
+  if (c < j.D) {
+    const float* p = j.sums + (ll)q * j.D + c;
+#pragma unroll 8
+    for (int k = w; k < j.parts; k += 32) t += p[(ll)k * kSums * j.D];
+  }
+  strand[w][x] = t;
   __syncthreads();
   if (w || c >= j.D) return;
-  t = (strand[0][threadIdx.x] + strand[1][threadIdx.x]) + (strand[2][threadIdx.x] + strand[3][threadIdx.x]);
-  if (q == kScale && j.scale_one)
+  t = 0.f;
+#pragma unroll
+  for (int k = 0; k < 32; k++) t += strand[k][x];
+  if (q == kScale && j.scale_cols)
     j.scale_cols[c] = t;
-  else if (j.rows32)
+  else if (j.w32)
     static_cast<float*>(j.out[q])[c] = t;
   else
     static_cast<T*>(j.out[q])[c] = (T)t;
@@ -418,7 +798,7 @@ __global__ __launch_bounds__(256) void resnorm_join_scale(const Join j) {
     __syncthreads();
   }
   if (threadIdx.x) return;
-  if (j.rows32)
+  if (j.w32)
     *static_cast<float*>(j.out[kScale]) = part[0];
   else
     *static_cast<T*>(j.out[kScale]) = (T)part[0];
@@ -434,19 +814,36 @@ struct DropArgs {
   mjh_i64* ctr_out;
 };
 
-template <class T, int V>
+// A stream of 16-byte pieces, V elements each; the words of a piece are one addition apart. A word costs two 64-bit
+// products, so a word for two elements keeps the arithmetic below the memory's time (at 50 million bfloat16
+// elements 40 us, 5.0 TB/s, about the rate of a copy of that size).
+template <class T>
 __global__ __launch_bounds__(256) void dropout_flat(const DropArgs a) {
+  constexpr int V = 16 / (int)sizeof(T);
   const unsigned long long base = drop_base(a.drop);
   if (a.ctr_out && blockIdx.x == 0 && threadIdx.x == 0) *a.ctr_out = a.drop.ctr ? *a.drop.ctr : 0;
   for (ll i = ((ll)blockIdx.x * 256 + threadIdx.x) * V; i < a.count; i += (ll)gridDim.x * 256 * V) {
-    const auto x = load<T, V>(static_cast<const T*>(a.x) + i);
-    float o[V];
+    const T* px = static_cast<const T*>(a.x) + i;
+    T* py = static_cast<T*>(a.y) + i;
+    unsigned long long z = base + (((unsigned long long)i >> 1) + 1ull) * 0x9e3779b97f4a7c15ull;
+    if (i + V <= a.count) {
+      const auto x = load_loose<T, V>(px);
+      float o[V];
 #pragma unroll
-    for (int j = 0; j < V; j++) {
-      const unsigned long long w = drop_word(base, (unsigned long long)(i + j) >> 1);
-      o[j] = drop_keep(w, V > 1 ? j & 1 : (int)((i + j) & 1), a.drop.thr) ? (float)x.v[j] * a.drop.scale : 0.f;
+      for (int j = 0; j < V; j += 2) {
+        const unsigned long long w = mjh::mix64(z);
+        o[j] = drop_keep(w, 0, a.drop.thr) ? (float)x.v[j] * a.drop.scale : 0.f;
+        o[j + 1] = drop_keep(w, 1, a.drop.thr) ? (float)x.v[j + 1] * a.drop.scale : 0.f;
+        z += 0x9e3779b97f4a7c15ull;
+      }
+      store_loose<T, V>(py, o);
+    } else {  // the last elements
+      for (int j = 0; i + j < a.count; j++) {
+        const unsigned long long w = mjh::mix64(z);
+        py[j] = (T)(drop_keep(w, j & 1, a.drop.thr) ? (float)px[j] * a.drop.scale : 0.f);
+        if (j & 1) z += 0x9e3779b97f4a7c15ull;
+      }
     }
-    store<T, V>(static_cast<T*>(a.y) + i, o);
   }
 }
 template <class T>
@@ -462,29 +859,30 @@ __global__ __launch_bounds__(256) void dropout_rows(const DropArgs a) {
 }
 
 // ---- host side ------------------------------------------------------------------------
-int tpr_of(int D) {
+// lanes that hold a row, and the workgroup that does: whole waves beyond one
+int lanes_of(int D) {
+  if (D > 64 * kPer) return (D + 64 * kPer - 1) / (64 * kPer) * 64;
   int t = 8;
   while (t * kPer < D) t *= 2;
   return t;
 }
 
-// 16-byte pieces need every row of every tensor aligned to them
-bool vectors(const mjh_resnorm_desc& d) {
-  const size_t e = d.dtype == MJH_F32 ? 4 : 2;
-  const ll v = 16 / (ll)e;
-  if (d.D % v) return false;
-  for (ll s : {d.ys, d.rs, d.gs, d.ss, d.ns, d.dss, d.dns, d.dys, d.drs, d.dgs})
-    if (s % v) return false;
-  for (const void* p : {d.y, d.r, d.gate, (const void*)d.s, (const void*)d.n, d.ds, d.dn, (const void*)d.dy,
-                        (const void*)d.dr, (const void*)d.dgate})
-    if (!aligned(p, 16)) return false;
-  return true;
+// the backward pass's parts write partial sums each, so a part takes several rows
+bool wide(int D) { return D > 256 * kPer; }
+unsigned parts_of(int D, ll rows, int dtype) {
+  const int lanes = lanes_of(D);
+  if (wide(D)) {
+    const ll tiles = (D + 64 * (dtype == MJH_F32 ? 4 : 8) - 1) / (64 * (dtype == MJH_F32 ? 4 : 8));
+    return (unsigned)std::max<ll>(1, std::min<ll>(rows / 4, kColumnWaves / tiles));
+  }
+  const ll groups = lanes > 64 ? 1 : 256 / lanes, waves = lanes > 64 ? lanes / 64 : 4;
+  return (unsigned)std::max<ll>(1, std::min<ll>((rows + groups - 1) / groups / 4, 256 * 12 / waves));
 }
 
 int check(const mjh_resnorm_desc* d) {
   if (!d) return refuse("residual norm: no description");
   if (d->R < 1 || d->D < 1) return refuse("residual norm: R and D must be positive");
-  if (d->D > kMaxTpr * kPer) return refuse("residual norm: D is at most 8192");
+  if (d->D > kMaxDim) return refuse("residual norm: D is at most 8192");
   if (d->R > 0x7fffffffll) return refuse("residual norm: R must be below 2^31");
   if (d->dtype < 0 || d->dtype > 2) return refuse("residual norm: unknown type");
   if (!d->r) return refuse("residual norm: the residual is needed");
@@ -513,48 +911,67 @@ Args args_of(const mjh_resnorm_desc& d) {
   a.drop = {d.seed, d.key, d.ctr, d.thr, d.thr ? d.drop_scale : 1.f};
   a.ctr_out = d.ctr_out;
   a.eps = d.eps;
+  a.inv = (float)(1.0 / d.D);
   a.R = (int)d.R; a.D = d.D; a.layer = d.layer; a.act = d.act; a.post = d.post; a.pre = d.pre;
+  a.tpr = lanes_of(d.D);
+  a.parts = (int)parts_of(d.D, d.R, d.dtype);
   return a;
 }
 
-unsigned grid_of(int tpr, ll rows, bool back) {
-  const int groups = block_of(tpr) / tpr;
+// rows of which a workgroup (a wave of the wide rows' column stream) takes one after another
+unsigned grid_of(int lanes, ll rows) {
+  const int groups = lanes > 64 ? 1 : 256 / lanes;
   const ll need = (rows + groups - 1) / groups;
-  if (!back) return (unsigned)std::min<ll>(need, 256 * 16);
-  // backward: workgroups write partial sums, so each takes several rows per group
-  return (unsigned)std::max<ll>(1, std::min<ll>(need / 8, 1024));
+  return (unsigned)std::min<ll>(need, 256 * 32 / (lanes > 64 ? lanes / 64 : 4));
 }
-
 bool wants_bias(const mjh_resnorm_desc& d) { return d.post_b || d.pre_b; }
 
-template <class T, bool VEC, int TPR>
-void launch_tpr(const Args& a, bool back, bool bias, hipStream_t s) {
-  const dim3 grid(grid_of(TPR, a.R, back)), block(block_of(TPR));
-  if (!back)
-    resnorm_forward<T, VEC, TPR><<<grid, block, 0, s>>>(a);
-  else if (a.y)
-    bias ? resnorm_backward<T, VEC, TPR, true, true><<<grid, block, 0, s>>>(a)
-         : resnorm_backward<T, VEC, TPR, true, false><<<grid, block, 0, s>>>(a);
-  else
-    bias ? resnorm_backward<T, VEC, TPR, false, true><<<grid, block, 0, s>>>(a)
-         : resnorm_backward<T, VEC, TPR, false, false><<<grid, block, 0, s>>>(a);
+template <class T, bool FULL, int TPR>
+void launch_forward(const Args& a, hipStream_t s) {
+  resnorm_forward<T, FULL, TPR><<<dim3(grid_of(a.tpr, a.R)), dim3(TPR > 64 ? a.tpr : 256), 0, s>>>(a);
 }
-template <class T, bool VEC>
-void launch_rows(const Args& a, bool back, bool bias, hipStream_t s) {
-  switch (tpr_of(a.D)) {
-    case 8: return launch_tpr<T, VEC, 8>(a, back, bias, s);
-    case 16: return launch_tpr<T, VEC, 16>(a, back, bias, s);
-    case 32: return launch_tpr<T, VEC, 32>(a, back, bias, s);
-    case 64: return launch_tpr<T, VEC, 64>(a, back, bias, s);
-    case 128: return launch_tpr<T, VEC, 128>(a, back, bias, s);
-    case 256: return launch_tpr<T, VEC, 256>(a, back, bias, s);
-    case 512: return launch_tpr<T, VEC, 512>(a, back, bias, s);
-    default: return launch_tpr<T, VEC, 1024>(a, back, bias, s);
-  }
+template <class T, bool FULL, int TPR, bool BLOCK, bool BIAS>
+void launch_backward(const Args& a, hipStream_t s) {
+  resnorm_backward<T, FULL, TPR, BLOCK, BIAS><<<dim3(a.parts), dim3(TPR > 64 ? a.tpr : 256), 0, s>>>(a);
+}
+template <class T, bool BLOCK, bool BIAS>
+void launch_wide(const Args& a, hipStream_t s) {
+  constexpr int N = 64 * Piece<T>::N;
+  resnorm_rows<T, BLOCK, BIAS><<<dim3(a.R), dim3(256), 0, s>>>(a);
+  resnorm_columns<T, BLOCK, BIAS><<<dim3((a.D + N - 1) / N, a.parts), dim3(64), 0, s>>>(a);
+}
+template <class T, bool FULL>
+void launch_forward_rows(const Args& a, hipStream_t s) {
+  // the fewest threads a workgroup is compiled for leave a lane the most registers
+  if (a.tpr == 8) return launch_forward<T, FULL, 8>(a, s);
+  if (a.tpr == 16) return launch_forward<T, FULL, 16>(a, s);
+  if (a.tpr == 32) return launch_forward<T, FULL, 32>(a, s);
+  if (a.tpr == 64) return launch_forward<T, FULL, 64>(a, s);
+  if (a.tpr <= 256) return launch_forward<T, FULL, 256>(a, s);
+  if (a.tpr <= 512) return launch_forward<T, FULL, 512>(a, s);
+  if (a.tpr <= 768) return launch_forward<T, FULL, 768>(a, s);
+  launch_forward<T, FULL, 1024>(a, s);
+}
+template <class T, bool FULL, bool BLOCK, bool BIAS>
+void launch_backward_rows(const Args& a, hipStream_t s) {
+  if (a.tpr == 8) return launch_backward<T, FULL, 8, BLOCK, BIAS>(a, s);
+  if (a.tpr == 16) return launch_backward<T, FULL, 16, BLOCK, BIAS>(a, s);
+  if (a.tpr == 32) return launch_backward<T, FULL, 32, BLOCK, BIAS>(a, s);
+  if (a.tpr == 64) return launch_backward<T, FULL, 64, BLOCK, BIAS>(a, s);
+  launch_backward<T, FULL, 256, BLOCK, BIAS>(a, s);
+}
+template <class T, bool BLOCK, bool BIAS>
+void launch_backward_as(const Args& a, hipStream_t s) {
+  if (wide(a.D)) return launch_wide<T, BLOCK, BIAS>(a, s);
+  a.tpr * kPer == a.D ? launch_backward_rows<T, true, BLOCK, BIAS>(a, s) : launch_backward_rows<T, false, BLOCK, BIAS>(a, s);
 }
 template <class T>
 void launch_type(const mjh_resnorm_desc& d, const Args& a, bool back, hipStream_t s) {
-  vectors(d) ? launch_rows<T, true>(a, back, wants_bias(d), s) : launch_rows<T, false>(a, back, wants_bias(d), s);
+  if (!back) return a.tpr * kPer == a.D ? launch_forward_rows<T, true>(a, s) : launch_forward_rows<T, false>(a, s);
+  if (a.y)
+    wants_bias(d) ? launch_backward_as<T, true, true>(a, s) : launch_backward_as<T, true, false>(a, s);
+  else
+    wants_bias(d) ? launch_backward_as<T, false, true>(a, s) : launch_backward_as<T, false, false>(a, s);
 }
 void launch(const mjh_resnorm_desc& d, const Args& a, bool back, hipStream_t s) {
   if (d.dtype == MJH_F32)
@@ -566,25 +983,19 @@ void launch(const mjh_resnorm_desc& d, const Args& a, bool back, hipStream_t s) 
 }
 
 template <class T>
-void launch_join(const Join& j, hipStream_t s) {
-  resnorm_join<T><<<dim3((j.D + 63) / 64, kSums), dim3(256), 0, s>>>(j);
-  if (j.scale_one && j.out[kScale]) resnorm_join_scale<T><<<dim3(1), dim3(256), 0, s>>>(j);
+void launch_join(const Join& j, int wanted, hipStream_t s) {
+  resnorm_join<T><<<dim3((j.D + 31) / 32, wanted), dim3(1024), 0, s>>>(j);
+  if (j.scale_cols && j.out[kScale]) resnorm_join_scale<T><<<dim3(1), dim3(256), 0, s>>>(j);
 }
 
 template <class T>
 void launch_dropout(const DropArgs& a, hipStream_t s) {
-  constexpr int V = 16 / (int)sizeof(T);
-  const ll most = 256 * 32;
-  if (a.rows == 1 && a.count % V == 0 && aligned(a.x, 16) && aligned(a.y, 16)) {
-    const ll n = (a.count / V + 255) / 256;
-    dropout_flat<T, V><<<dim3((unsigned)std::min(n, most)), dim3(256), 0, s>>>(a);
-  } else {
-    const ll n = (a.count + 255) / 256;
-    if (a.rows == 1)
-      dropout_flat<T, 1><<<dim3((unsigned)std::min(n, most)), dim3(256), 0, s>>>(a);
-    else
-      dropout_rows<T><<<dim3((unsigned)std::min(n, most)), dim3(256), 0, s>>>(a);
-  }
+  const ll most = 256 * 32, per = a.rows == 1 ? 256 * 16 / (ll)sizeof(T) : 256;
+  const dim3 grid((unsigned)std::min((a.count + per - 1) / per, most));
+  if (a.rows == 1)
+    dropout_flat<T><<<grid, dim3(256), 0, s>>>(a);
+  else
+    dropout_rows<T><<<grid, dim3(256), 0, s>>>(a);
 }
 
 }  // namespace
@@ -593,7 +1004,8 @@ extern "C" {
 
 long long mjh_resnorm_workspace(const mjh_resnorm_desc* d) {
   if (check(d)) return -1;
-  return 4 * ((ll)grid_of(tpr_of(d->D), d->R, true) * kSums * d->D + d->D);
+  // partial sums, the scale's column sums, the row sums of wide rows (first: 16-byte aligned)
+  return 4 * ((wide(d->D) ? 4 * d->R : 0) + (ll)parts_of(d->D, d->R, d->dtype) * kSums * d->D + d->D);
 }
 
 int mjh_resnorm_forward(const mjh_resnorm_desc* d, void* stream) {
@@ -607,29 +1019,33 @@ int mjh_resnorm_backward(const mjh_resnorm_desc* d, void* stream) {
   if (int rc = check(d)) return rc;
   if (!d->stats || (!d->ds && !d->dn) || (d->dn && !d->pre)) return refuse("residual norm backward: statistics or gradients are missing");
   const bool sums = d->d_post_w || d->d_post_b || d->d_scale || d->d_pre_w || d->d_pre_b;
-  if (sums && (!d->ws || d->ws_bytes < mjh_resnorm_workspace(d))) return refuse("residual norm backward: workspace too small");
+  if ((sums || wide(d->D)) && (!d->ws || d->ws_bytes < mjh_resnorm_workspace(d)))
+    return refuse("residual norm backward: workspace too small");
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   Args a = args_of(*d);
-  a.sums = sums ? static_cast<float*>(d->ws) : nullptr;
+  a.coef = static_cast<float*>(d->ws);
+  a.sums = sums ? static_cast<float*>(d->ws) + (wide(a.D) ? 4 * (ll)a.R : 0) : nullptr;
   launch(*d, a, true, s);
   if (int rc = launched()) return rc;
   if (!sums) return 0;
   Join j;
   std::memset(&j, 0, sizeof(j));
   j.sums = a.sums;
-  j.parts = (int)grid_of(tpr_of(a.D), a.R, true);
+  j.parts = a.parts;
   j.D = a.D;
-  j.rows32 = a.w32;
+  j.w32 = a.w32;
   j.out[kPostW] = d->d_post_w; j.out[kPostB] = d->d_post_b; j.out[kScale] = d->d_scale;
   j.out[kPreW] = d->d_pre_w; j.out[kPreB] = d->d_pre_b;
-  j.scale_one = a.scale_one;
-  j.scale_cols = a.sums + (ll)j.parts * kSums * a.D;
+  int wanted = 0;
+  for (int q = 0; q < kSums; q++)
+    if (j.out[q]) j.q[wanted++] = q;
+  if (a.scale_one) j.scale_cols = a.sums + (ll)j.parts * kSums * a.D;
   if (d->dtype == MJH_F32)
-    launch_join<float>(j, s);
+    launch_join<float>(j, wanted, s);
   else if (d->dtype == MJH_BF16)
-    launch_join<bf16>(j, s);
+    launch_join<bf16>(j, wanted, s);
   else
-    launch_join<f16>(j, s);
+    launch_join<f16>(j, wanted, s);
   return launched();
 }
 

@@ -16,7 +16,7 @@
 // x, which the blend needs anyway, is not joined by a second stream.
 //
 // With few channels the steps are cut into chunks: one launch forms each chunk's (product of a, result from 0),
-// and the main launch joins those of the chunks before its own.
+// a second joins them into the state that comes into each chunk, and the main launch starts from that.
 #include <algorithm>
 #include <cstring>
 #include <type_traits>
@@ -57,15 +57,17 @@ struct Args {
 
 struct Where {
   int n, d, g;
-  bool on;
+  bool on;   // there are channels here
+  bool row;  // heads: the head exists (a lane beside its channels may still end up with a step's sum)
 };
 
 // Channels flat over (row, vector): consecutive lanes read consecutive addresses across row ends too.
 template <int V>
 __device__ __forceinline__ Where flat_where(const Args& a) {
-  const unsigned i = blockIdx.x * kBlock + threadIdx.x;
+  unsigned i = blockIdx.x * kBlock + threadIdx.x;
   Where w;
-  w.on = i < (unsigned)a.N * (unsigned)a.dv;
+  w.on = w.row = i < (unsigned)a.N * (unsigned)a.dv;
+  if (!w.on) i = (unsigned)a.N * (unsigned)a.dv - 1;
   w.n = (int)(i / (unsigned)a.dv);
   w.d = (int)(i - (unsigned)w.n * (unsigned)a.dv) * V;
   w.g = a.K == 1 ? w.d : w.d / a.K;
@@ -89,7 +91,9 @@ __device__ __forceinline__ Where head_where(const Args& a, int& lane_in_head, in
   }
   Where w;
   const int c = (part * 64 + lane_in_head) * V;
-  w.on = slot < (unsigned)a.N * (unsigned)a.G && c < a.K;
+  w.row = slot < (unsigned)a.N * (unsigned)a.G;
+  w.on = w.row && c < a.K;
+  if (!w.row) slot = (unsigned)a.N * (unsigned)a.G - 1;
   w.n = (int)(slot / (unsigned)a.G);
   w.g = (int)(slot % (unsigned)a.G);
   w.d = w.g * a.K + c;
@@ -111,230 +115,411 @@ struct Gate {
   }
 };
 
-// The float32 state before chunk c (forward: from the first chunk on; backward: gradient after chunk c, from
-// the last on). A chunk with a reset inside passes nothing on, whatever comes in (not 0 times it: the state
-// before a reset may be infinite or NaN).
-template <int V, bool BACK>
-__device__ __forceinline__ void join_chunks(const Args& a, const Where& w, int c, float (&s)[V]) {
-  const ll nd = (ll)a.N * a.D, at = (ll)w.n * a.D + w.d;
-  for (int k = BACK ? a.nchunk - 1 : 0; BACK ? k > c : k < c; BACK ? k-- : k++) {
-    const auto p = load<float, V>(a.agg_a + k * nd + at);
-    const auto q = load<float, V>(a.agg_b + k * nd + at);
-    const bool cut = a.reset && a.agg_cut[(ll)k * a.N + w.n];
+// The chunks' results become the state that comes into each chunk (forward: from the chunks before it; BACK: the
+// gradient from the chunks after it), written over the chunk's own result in agg_b. A workgroup holds 64 channels
+// by 16 waves; a wave takes kJoin neighbouring chunks, all loads in flight at once (one thread a channel and a loop
+// over 256 chunks took 70 us, this 5). A chunk with a reset inside passes nothing on, whatever comes in (not 0 times
+// it: the state before a reset may be infinite or NaN).
+constexpr int kJoin = 16, kMaxChunks = 16 * kJoin;
+template <bool BACK>
+__global__ __launch_bounds__(1024) void scan_join(const Args a) {
+  __shared__ float sa[16][64], sb[16][64];
+  __shared__ unsigned char sc[16][64];
+  const ll nd = (ll)a.N * a.D, at = (ll)blockIdx.x * 64 + (threadIdx.x & 63);
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const bool on = at < nd;
+  const int n = on ? (int)(at / a.D) : 0;
+  const float* edge = BACK ? a.dlast : a.state;
+  const float first = on && edge ? edge[at] : 0.f;
+  float p[kJoin], q[kJoin];
+  bool cut[kJoin];
 #pragma unroll
-    for (int v = 0; v < V; v++) s[v] = cut ? q.v[v] : __builtin_fmaf(p.v[v], s[v], q.v[v]);
+  for (int k = 0; k < kJoin; k++) {
+    const int i = w * kJoin + k;  // in the order of the recurrence
+    const bool in = on && i < a.nchunk;
+    const int c = in ? (BACK ? a.nchunk - 1 - i : i) : 0;
+    p[k] = in ? a.agg_a[c * nd + at] : 1.f;
+    q[k] = in ? a.agg_b[c * nd + at] : 0.f;
+    cut[k] = in && a.reset && a.agg_cut[(ll)c * a.N + n];
+  }
+  float ta = 1.f, tb = 0.f;
+  bool tc = false;
+#pragma unroll
+  for (int k = 0; k < kJoin; k++) {
+    tb = cut[k] ? q[k] : __builtin_fmaf(p[k], tb, q[k]);
+    ta *= p[k];
+    tc |= cut[k];
+  }
+  sa[w][lane] = ta;
+  sb[w][lane] = tb;
+  sc[w][lane] = tc;
+  __syncthreads();
+  float s = first;
+  for (int k = 0; k < w; k++) s = sc[k][lane] ? sb[k][lane] : __builtin_fmaf(sa[k][lane], s, sb[k][lane]);
+#pragma unroll
+  for (int k = 0; k < kJoin; k++) {
+    const int i = w * kJoin + k;
+    if (!on || i >= a.nchunk) break;
+    a.agg_b[(BACK ? a.nchunk - 1 - i : i) * nd + at] = s;
+    s = cut[k] ? q[k] : __builtin_fmaf(p[k], s, q[k]);
   }
 }
 
-template <class T, class GT, int V, int GV>
-struct Block {
-  Pack<T, V> x[kSteps];
-  Pack<GT, GV> g[kSteps];
-  unsigned char r[kSteps];
+// The state (BACK: gradient) that comes into chunk c.
+template <int V, bool BACK>
+__device__ __forceinline__ void incoming(const Args& a, ll at, int c, float (&s)[V]) {
+  const float* from = a.nchunk > 1 ? a.agg_b + c * ((ll)a.N * a.D) : BACK ? a.dlast : a.state;
+#pragma unroll
+  for (int v = 0; v < V; v++) s[v] = 0.f;
+  if (!from) return;
+  const auto p = load<float, V>(from + at);
+#pragma unroll
+  for (int v = 0; v < V; v++) s[v] = p.v[v];
+}
 
-  // steps tb .. tb + kSteps; those from `end` on read step end - 1 again and are not used
-  template <bool WITH_X>
-  __device__ __forceinline__ void read(const Args& a, const Where& w, int tb, int end) {
+// A wave's place in the (T, N) reset flags. Where its rows are at most 8 neighbours (D of 16 and more), one load
+// brings the flags of kSteps steps for all of them: lane l reads step l % 8 of row l / 8, and a ballot hands every
+// lane its row's bits (a load per step and lane took 8 us of the 96 us of a 24 x 4,096 x 256 training pass).
+struct Flags {
+  int n0;
+  bool wide;
+  __device__ __forceinline__ explicit Flags(const Where& w) {
+    n0 = __builtin_amdgcn_readfirstlane(w.n);
+    wide = __builtin_amdgcn_readlane(w.n, 63) - n0 < 8;
+  }
+  // called by all lanes of the wave
+  __device__ __forceinline__ unsigned raw(const Args& a, const Where& w, int tb, int end) const {
+    static_assert(kSteps == 8, "8 steps by 8 rows fill a wave");
+    if (!a.reset) return 0;
+    if (wide) {
+      const int lane = threadIdx.x & 63;
+      return a.reset[(ll)min(tb + (lane & 7), end - 1) * a.rt + (ll)min(n0 + (lane >> 3), a.N - 1) * a.rn];
+    }
+    unsigned bits = 0;
+    for (int j = 0; j < kSteps; j++) bits |= (unsigned)(a.reset[(ll)min(tb + j, end - 1) * a.rt + (ll)w.n * a.rn] != 0) << j;
+    return bits;
+  }
+  __device__ __forceinline__ unsigned bits(const Args& a, const Where& w, unsigned raw) const {
+    if (!a.reset) return 0;
+    return wide ? (unsigned)(__ballot(raw != 0) >> (8 * (w.n - n0))) & 255u : raw;
+  }
+};
+
+// What a thread reads for kSteps steps from tb on; steps from `end` on read step end - 1 again and are not used.
+// Lanes with nothing to read (`on` false) take part for the flags.
+template <class T, class GT, int V, int GV, bool X, bool DH>
+struct Block {
+  Pack<T, V> x[kSteps], dh[kSteps];
+  Pack<GT, GV> g[kSteps];
+  unsigned flags;
+
+  __device__ __forceinline__ void read(const Args& a, const Where& w, const Flags& f, bool on, int tb, int end) {
+    flags = f.raw(a, w, tb, end);
+    if (!on) return;
     const T* px = static_cast<const T*>(a.x) + (ll)w.n * a.xn + w.d;
     const GT* pg = static_cast<const GT*>(a.gate) + (ll)w.n * a.gn + w.g;
+    const T* pd = static_cast<const T*>(a.dh) + (ll)w.n * a.dhn + w.d;
 #pragma unroll
     for (int j = 0; j < kSteps; j++) {
       const ll t = min(tb + j, end - 1);
-      if constexpr (WITH_X) x[j] = load<T, V>(px + t * a.xt);
+      if constexpr (X) x[j] = load<T, V>(px + t * a.xt);
       g[j] = load<GT, GV>(pg + t * a.gt);
-      r[j] = 0;
     }
-    if (a.reset) {
-      const unsigned char* pr = a.reset + (ll)w.n * a.rn;
+    if constexpr (DH) {
+      if (a.dh) {
 #pragma unroll
-      for (int j = 0; j < kSteps; j++) r[j] = pr[(ll)min(tb + j, end - 1) * a.rt];
+        for (int j = 0; j < kSteps; j++) dh[j] = load<T, V>(pd + (ll)min(tb + j, end - 1) * a.dht);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kSteps; j++) dh[j] = Pack<T, V>{};
+      }
     }
   }
 };
 
-// AGG: the chunk's (product of a, result from state 0); else the outputs.
-template <class T, class GT, int V, int GV, bool BLEND, bool AGG>
+// the largest value of the wave's lanes, the same in all
+__device__ __forceinline__ int wave_max(int v) {
+#pragma unroll
+  for (int m = 32; m > 0; m >>= 1) v = max(v, __shfl_xor(v, m));
+  return __builtin_amdgcn_readfirstlane(v);
+}
+
+// AGG: the chunk's (product of a, result from state 0); else the outputs. AHEAD: loads of the next block under way
+// while this one is worked on, for chunked launches; with a thread for every channel of many rows the waves that
+// its registers cost are worth more.
+template <class T, class GT, int V, int GV, bool BLEND, bool AGG, bool AHEAD>
 __global__ __launch_bounds__(kBlock) void scan_forward(const Args a) {
   const Where w = flat_where<V>(a);
-  if (!w.on) return;
+  const Flags flags(w);
   const int c = blockIdx.y, t0 = c * a.chunk, t1 = min(a.T, t0 + a.chunk);
-  const int live = a.lengths ? min(a.lengths[w.n], t1) : t1;
+  const int live = !w.on ? 0 : a.lengths ? min(a.lengths[w.n], t1) : t1;
+  const int stop = a.lengths ? wave_max(live) : t1;  // the same in all lanes, as every read and ballot needs
   const ll nd = (ll)a.N * a.D, at = (ll)w.n * a.D + w.d;
   float s[V], prod[V];
 #pragma unroll
   for (int v = 0; v < V; v++) s[v] = 0.f, prod[v] = 1.f;
   bool cut = false;
-  if (!AGG) {
-    if (a.state) {
-      const auto p = load<float, V>(a.state + at);
-#pragma unroll
-      for (int v = 0; v < V; v++) s[v] = p.v[v];
-    }
-    join_chunks<V, false>(a, w, c, s);
-  }
+  if (!AGG) incoming<V, false>(a, at, c, s);
   T* ph = static_cast<T*>(a.h) + (ll)w.n * a.hn + w.d;
-  for (int tb = t0; tb < t1; tb += kSteps) {
-    Block<T, GT, V, GV> b;
-    b.template read<true>(a, w, tb, t1);
-    if (!AGG && a.kept) store<float, V>(a.kept + (ll)(tb / kSteps) * nd + at, s);
+  Block<T, GT, V, GV, true, false> b, next;
+  if (AHEAD && t0 < stop) b.read(a, w, flags, t0 < live, t0, t1);
+  int tb = t0;
+  for (; tb < stop; tb += kSteps) {
+    if (!AGG && a.kept && w.on) store<float, V>(a.kept + (ll)(tb / kSteps) * nd + at, s);
+    if (!AHEAD) b.read(a, w, flags, tb < live, tb, t1);
+    if (AHEAD && tb + kSteps < stop) next.read(a, w, flags, tb + kSteps < live, tb + kSteps, t1);
+    const unsigned bits = flags.bits(a, w, b.flags);
+    if (__all(bits == 0 && tb + kSteps <= live)) {
 #pragma unroll
-    for (int j = 0; j < kSteps; j++) {
-      const int t = tb + j;
-      if (t >= t1) break;
-      const bool in = t < live;
-      float out[V];
+      for (int j = 0; j < kSteps; j++) {
+        float out[V];
 #pragma unroll
-      for (int v = 0; v < V; v++) {
-        const Gate<BLEND> f((float)b.g[j].v[GV == 1 ? 0 : v]);
-        const float x = (float)b.x[j].v[v];
-        const float add = BLEND ? f.b * x : x;
-        const float next = b.r[j] ? add : __builtin_fmaf(f.a, s[v], add);
-        if (AGG) prod[v] = in ? (b.r[j] ? 0.f : prod[v] * f.a) : prod[v];
-        s[v] = in ? next : s[v];
-        out[v] = in ? next : 0.f;
+        for (int v = 0; v < V; v++) {
+          const Gate<BLEND> f((float)b.g[j].v[GV == 1 ? 0 : v]);
+          const float x = (float)b.x[j].v[v];
+          out[v] = s[v] = __builtin_fmaf(f.a, s[v], BLEND ? f.b * x : x);
+          if (AGG) prod[v] *= f.a;
+        }
+        if (!AGG) store<T, V>(ph + (ll)(tb + j) * a.ht, out);
       }
-      if (AGG) cut |= in && b.r[j];
-      if (!AGG) store<T, V>(ph + (ll)t * a.ht, out);
+    } else {  // a reset, a row's end or the last step inside
+#pragma unroll
+      for (int j = 0; j < kSteps; j++) {
+        const bool in = tb + j < live, reset = bits >> j & 1u;
+        float out[V];
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+          out[v] = 0.f;
+          if (in) {
+            const Gate<BLEND> f((float)b.g[j].v[GV == 1 ? 0 : v]);
+            const float x = (float)b.x[j].v[v];
+            out[v] = s[v] = __builtin_fmaf(f.a, reset ? 0.f : s[v], BLEND ? f.b * x : x);
+            if (AGG) prod[v] = reset ? 0.f : prod[v] * f.a;
+          }
+        }
+        if (AGG) cut |= in && reset;
+        if (!AGG && w.on && tb + j < t1) store<T, V>(ph + (ll)(tb + j) * a.ht, out);
+      }
     }
+    if (AHEAD) b = next;
   }
+  if (!w.on) return;
   if (AGG) {
     store<float, V>(a.agg_a + c * nd + at, prod);
     store<float, V>(a.agg_b + c * nd + at, s);
     if (a.reset && w.d == 0) a.agg_cut[(ll)c * a.N + w.n] = cut;
-  } else if (c == a.nchunk - 1) {
-    store<float, V>(a.last + at, s);
+    return;
   }
+  for (; tb < t1; tb += kSteps) {  // beyond the rows' lengths: nothing to read
+    if (a.kept) store<float, V>(a.kept + (ll)(tb / kSteps) * nd + at, s);
+    const float none[V] = {};
+#pragma unroll
+    for (int j = 0; j < kSteps; j++)
+      if (tb + j < t1) store<T, V>(ph + (ll)(tb + j) * a.ht, none);
+  }
+  if (c == a.nchunk - 1) store<float, V>(a.last + at, s);
 }
 
 // The chunk's effect on the gradient that comes in from the steps after it.
 template <class T, class GT, int V, int GV, bool BLEND>
 __global__ __launch_bounds__(kBlock) void scan_backward_agg(const Args a) {
   const Where w = flat_where<V>(a);
-  if (!w.on) return;
+  const Flags flags(w);
   const int c = blockIdx.y, t0 = c * a.chunk, t1 = min(a.T, t0 + a.chunk);
-  const int live = a.lengths ? min(a.lengths[w.n], t1) : t1;
+  const int live = !w.on ? 0 : a.lengths ? min(a.lengths[w.n], t1) : t1;
+  const int stop = a.lengths ? wave_max(live) : t1;
   const ll nd = (ll)a.N * a.D, at = (ll)w.n * a.D + w.d;
-  const T* pd = static_cast<const T*>(a.dh) + (ll)w.n * a.dhn + w.d;
   float e[V], prod[V];
 #pragma unroll
   for (int v = 0; v < V; v++) e[v] = 0.f, prod[v] = 1.f;
   bool cut = false;
-  for (int tb = t0 + (t1 - 1 - t0) / kSteps * kSteps; tb >= t0; tb -= kSteps) {
-    Block<T, GT, V, GV> b;
-    b.template read<false>(a, w, tb, t1);
-    Pack<T, V> dh[kSteps];
+  if (stop > t0) {
+    Block<T, GT, V, GV, false, true> b, next;
+    int tb = t0 + (stop - 1 - t0) / kSteps * kSteps;
+    b.read(a, w, flags, tb < live, tb, t1);
+    for (; tb >= t0; tb -= kSteps) {
+      if (tb > t0) next.read(a, w, flags, tb - kSteps < live, tb - kSteps, t1);
+      const unsigned bits = flags.bits(a, w, b.flags);
+      if (__all(bits == 0 && tb + kSteps <= live)) {
 #pragma unroll
-    for (int j = 0; j < kSteps; j++) {
-      if (a.dh)
-        dh[j] = load<T, V>(pd + (ll)min(tb + j, t1 - 1) * a.dht);
-      else
-        dh[j] = Pack<T, V>{};
-    }
+        for (int j = kSteps - 1; j >= 0; j--)
 #pragma unroll
-    for (int j = kSteps - 1; j >= 0; j--) {
-      const int t = tb + j;
-      if (t >= live) continue;
+          for (int v = 0; v < V; v++) {
+            const Gate<BLEND> f((float)b.g[j].v[GV == 1 ? 0 : v]);
+            e[v] = f.a * ((float)b.dh[j].v[v] + e[v]);
+            prod[v] *= f.a;
+          }
+      } else {
 #pragma unroll
-      for (int v = 0; v < V; v++) {
-        const Gate<BLEND> f((float)b.g[j].v[GV == 1 ? 0 : v]);
-        e[v] = b.r[j] ? 0.f : f.a * ((float)dh[j].v[v] + e[v]);
-        prod[v] = b.r[j] ? 0.f : prod[v] * f.a;
+        for (int j = kSteps - 1; j >= 0; j--) {
+          if (tb + j >= live) continue;
+          const bool reset = bits >> j & 1u;
+#pragma unroll
+          for (int v = 0; v < V; v++) {
+            const Gate<BLEND> f((float)b.g[j].v[GV == 1 ? 0 : v]);
+            e[v] = reset ? 0.f : f.a * ((float)b.dh[j].v[v] + e[v]);
+            prod[v] = reset ? 0.f : prod[v] * f.a;
+          }
+          cut |= reset;
+        }
       }
-      cut |= b.r[j] != 0;
+      b = next;
     }
   }
+  if (!w.on) return;
   store<float, V>(a.agg_a + c * nd + at, prod);
   store<float, V>(a.agg_b + c * nd + at, e);
   if (a.reset && w.d == 0) a.agg_cut[(ll)c * a.N + w.n] = cut;
 }
 
-// HEADS: dgate is summed over a head's lanes (a butterfly: a fixed order).
+// kSteps values summed over groups of `lanes` lanes (a power of two). While a lane holds several steps it hands
+// half of them to its partner and takes the other half's terms (4 + 2 + 1 exchanges for 8 steps where summing each
+// step by itself takes 8 at every level). Returns the first step this lane ends with; `count` steps are left in
+// v[0..], the same in the lanes that differ in the bits of `same` only. A fixed order: no run differs from another.
+__device__ __forceinline__ int sum_over_lanes(float (&v)[kSteps], int lane, int lanes, int& count, int& same) {
+  int m = lanes >> 1, base = 0;
+  count = kSteps;
+#pragma unroll
+  for (int n = kSteps; n > 1; n /= 2) {
+    if (m > 0) {
+      const bool up = lane & m;
+#pragma unroll
+      for (int i = 0; i < n / 2; i++) {
+        const float send = up ? v[i] : v[i + n / 2], mine = up ? v[i + n / 2] : v[i];
+        v[i] = mine + __shfl_xor(send, m);
+      }
+      base += up ? n / 2 : 0;
+      count = n / 2;
+      m >>= 1;
+    }
+  }
+  same = m ? 2 * m - 1 : 0;
+  for (; m > 0; m >>= 1) v[0] += __shfl_xor(v[0], m);
+  return base;
+}
+
+// HEADS: dgate is summed over a head's lanes; lanes beside its channels take part with 0.
 template <class T, class GT, int V, int GV, bool BLEND, bool HEADS>
 __global__ __launch_bounds__(kBlock) void scan_backward(const Args a) {
   int lane = 0, part = 0;
   const Where w = HEADS ? head_where<V>(a, lane, part) : flat_where<V>(a);
-  if (!HEADS && !w.on) return;
-  const bool on = w.on;  // lanes beside a head's channels take part in its sums with 0
+  const Flags flags(w);
+  const bool on = w.on;
   const int c = blockIdx.y, t0 = c * a.chunk, t1 = min(a.T, t0 + a.chunk);
   const ll nd = (ll)a.N * a.D, at = (ll)w.n * a.D + w.d;
   const int live = !on ? 0 : a.lengths ? min(a.lengths[w.n], t1) : t1;
+  const int stop = a.lengths ? wave_max(live) : t1;
   float e[V];
 #pragma unroll
   for (int v = 0; v < V; v++) e[v] = 0.f;
-  if (on) {
-    if (a.dlast) {
-      const auto p = load<float, V>(a.dlast + at);
-#pragma unroll
-      for (int v = 0; v < V; v++) e[v] = p.v[v];
-    }
-    join_chunks<V, true>(a, w, c, e);
-  }
-  const T* pd = static_cast<const T*>(a.dh) + (ll)w.n * a.dhn + w.d;
+  if (on) incoming<V, true>(a, at, c, e);
   T* px = static_cast<T*>(a.dx) + (ll)w.n * a.dxn + w.d;
   GT* pg = static_cast<GT*>(a.dgate) + (ll)w.n * a.dgn + w.g;
-  for (int tb = t0 + (t1 - 1 - t0) / kSteps * kSteps; tb >= t0; tb -= kSteps) {
-    Block<T, GT, V, GV> b;
-    Pack<T, V> dh[kSteps];
-    float before[kSteps][V];
-    if (on) {
-      b.template read<true>(a, w, tb, t1);
-      const auto k = load<float, V>(a.kept + (ll)(tb / kSteps) * nd + at);
-#pragma unroll
-      for (int j = 0; j < kSteps; j++) {
-        if (a.dh)
-          dh[j] = load<T, V>(pd + (ll)min(tb + j, t1 - 1) * a.dht);
-        else
-          dh[j] = Pack<T, V>{};
-      }
-      float s[V];
+  const int last = t0 + (t1 - 1 - t0) / kSteps * kSteps;
+  Block<T, GT, V, GV, true, true> b, next;
+  Pack<float, V> k, nextk;
+  auto fetch = [&](Block<T, GT, V, GV, true, true>& to, Pack<float, V>& tok, int tb) {
+    if (tb < t0 || tb >= stop) return;  // beyond the rows' lengths: nothing to read
+    to.read(a, w, flags, tb < live, tb, t1);
+    if (tb < live) tok = load<float, V>(a.kept + (ll)(tb / kSteps) * nd + at);
+  };
+  fetch(b, k, last);
+  for (int tb = last; tb >= t0; tb -= kSteps) {
+    fetch(next, nextk, tb - kSteps);  // under way while this block is worked on
+    float sum[kSteps];
+    const unsigned bits = tb < stop ? flags.bits(a, w, b.flags) : 0u;
+    if (__all(bits == 0 && tb + kSteps <= live)) {
+      // the states before each step, forward from the kept one; then the steps backward
+      float fa[kSteps][GV], fb[kSteps][GV], before[kSteps][V], s[V];
 #pragma unroll
       for (int v = 0; v < V; v++) s[v] = k.v[v];
 #pragma unroll
       for (int j = 0; j < kSteps; j++) {
 #pragma unroll
+        for (int v = 0; v < GV; v++) {
+          const Gate<BLEND> f((float)b.g[j].v[v]);
+          fa[j][v] = f.a;
+          fb[j][v] = f.b;
+        }
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+          const float x = (float)b.x[j].v[v];
+          before[j][v] = s[v];
+          s[v] = __builtin_fmaf(fa[j][GV == 1 ? 0 : v], s[v], BLEND ? fb[j][GV == 1 ? 0 : v] * x : x);
+        }
+      }
+#pragma unroll
+      for (int j = kSteps - 1; j >= 0; j--) {
+        float dx[V], dg[V];
+        sum[j] = 0.f;
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+          const float ga = fa[j][GV == 1 ? 0 : v], gb = fb[j][GV == 1 ? 0 : v];
+          const float delta = (float)b.dh[j].v[v] + e[v];
+          dx[v] = BLEND ? gb * delta : delta;
+          dg[v] = BLEND ? dx[v] * ga * (before[j][v] - (float)b.x[j].v[v]) : delta * before[j][v];
+          e[v] = ga * delta;
+          sum[j] += dg[v];
+        }
+        if (a.dx) store<T, V>(px + (ll)(tb + j) * a.dxt, dx);
+        if constexpr (!HEADS)
+          if (a.dgate) store<GT, V>(pg + (ll)(tb + j) * a.dgt, dg);
+      }
+    } else {  // a reset, a row's end, the last step, or lanes beside a head's channels
+      float s[V], before[kSteps][V];
+#pragma unroll
+      for (int v = 0; v < V; v++) s[v] = k.v[v];
+#pragma unroll
+      for (int j = 0; j < kSteps; j++) {
+        if (tb + j >= live) continue;
+#pragma unroll
         for (int v = 0; v < V; v++) {
           const Gate<BLEND> f((float)b.g[j].v[GV == 1 ? 0 : v]);
           const float x = (float)b.x[j].v[v];
-          before[j][v] = b.r[j] ? 0.f : s[v];
-          s[v] = b.r[j] ? f.b * x : __builtin_fmaf(f.a, s[v], f.b * x);
+          before[j][v] = bits >> j & 1u ? 0.f : s[v];
+          s[v] = __builtin_fmaf(f.a, before[j][v], BLEND ? f.b * x : x);
+        }
+      }
+#pragma unroll
+      for (int j = kSteps - 1; j >= 0; j--) {
+        float dx[V], dg[V];
+        sum[j] = 0.f;
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+          dx[v] = dg[v] = 0.f;
+          if (tb + j < live) {
+            const Gate<BLEND> f((float)b.g[j].v[GV == 1 ? 0 : v]);
+            const float delta = (float)b.dh[j].v[v] + e[v];
+            dx[v] = BLEND ? f.b * delta : delta;
+            dg[v] = BLEND ? dx[v] * f.a * (before[j][v] - (float)b.x[j].v[v]) : delta * before[j][v];
+            e[v] = bits >> j & 1u ? 0.f : f.a * delta;
+          }
+          sum[j] += dg[v];
+        }
+        if (on && tb + j < t1) {
+          if (a.dx) store<T, V>(px + (ll)(tb + j) * a.dxt, dx);
+          if constexpr (!HEADS)
+            if (a.dgate) store<GT, V>(pg + (ll)(tb + j) * a.dgt, dg);
         }
       }
     }
-#pragma unroll
-    for (int j = kSteps - 1; j >= 0; j--) {
-      const int t = tb + j;
-      if (t >= t1) continue;
-      const bool in = t < live;
-      float dx[V], dg[V], sum = 0.f;
-#pragma unroll
-      for (int v = 0; v < V; v++) {
-        dx[v] = dg[v] = 0.f;
-        if (in) {
-          const Gate<BLEND> f((float)b.g[j].v[GV == 1 ? 0 : v]);
-          const float delta = (float)dh[j].v[v] + e[v];
-          if (BLEND) {
-            dx[v] = f.b * delta;
-            dg[v] = dx[v] * f.a * (before[j][v] - (float)b.x[j].v[v]);
-          } else {
-            dx[v] = delta;
-            dg[v] = delta * before[j][v];
-          }
-          e[v] = b.r[j] ? 0.f : f.a * delta;
-        }
-        sum += dg[v];
-      }
-      if (a.dx && on) store<T, V>(px + (ll)t * a.dxt, dx);
+    b = next;
+    k = nextk;
+    if constexpr (HEADS) {
       if (a.dgate) {
-        if constexpr (HEADS) {
-          for (int m = a.lanes >> 1; m > 0; m >>= 1) sum += __shfl_xor(sum, m);
-          if (on && lane == 0) {
-            if (a.waves == 1)
-              pg[(ll)t * a.dgt] = (GT)sum;
-            else
-              a.part[(((ll)t * a.N + w.n) * a.G + w.g) * a.waves + part] = sum;
+        int count, same;
+        const int first = sum_over_lanes(sum, lane, a.lanes, count, same);
+        if (w.row && !(lane & same)) {
+#pragma unroll
+          for (int i = 0; i < kSteps; i++) {
+            const int t = tb + first + i;
+            if (i < count && t < t1) {
+              if (a.waves == 1)
+                pg[(ll)t * a.dgt] = (GT)sum[i];
+              else
+                a.part[(((ll)t * a.N + w.n) * a.G + w.g) * a.waves + part] = sum[i];
+            }
           }
-        } else {
-          store<GT, V>(pg + (ll)t * a.dgt, dg);
         }
       }
     }
@@ -380,11 +565,26 @@ enum Kernel { kForward, kForwardAgg, kBackward, kBackwardAgg, kStep };
 
 struct Plan {
   Args a;
-  int v;         // channels per thread
-  bool heads;    // gates shared by channels
+  bool heads;            // gates shared by channels
+  int v;                 // channels per thread of the launch at hand
   unsigned blocks;       // flat mapping
   unsigned head_blocks;  // head mapping
 };
+
+// Channels per thread: the launch's geometry.
+void set_width(Plan& p, int v) {
+  Args& a = p.a;
+  p.v = v;
+  a.dv = a.D / v;
+  p.blocks = (unsigned)(((ll)a.N * a.dv + kBlock - 1) / kBlock);
+  const int per = (a.K + v - 1) / v;  // lanes a head needs
+  a.lanes = 1;
+  while (a.lanes < per && a.lanes < 64) a.lanes *= 2;
+  a.waves = (per + 63) / 64;
+  const ll slots = (ll)a.N * a.G;
+  const ll waves = a.waves == 1 ? (slots + 64 / a.lanes - 1) / (64 / a.lanes) : slots * a.waves;
+  p.head_blocks = (unsigned)((waves + 3) / 4);
+}
 
 size_t type_size(int t) { return t == MJH_F32 ? 4 : 2; }
 
@@ -408,7 +608,10 @@ bool fits(const mjh_scan_desc& s, int v) {
   return true;
 }
 
-int make_plan(const mjh_scan_desc* s, bool back, Plan& p) {
+constexpr int kWide = 2;
+constexpr ll kThreads = 262144, kFull = 65536, kLeast = 4;
+
+int make_plan(const mjh_scan_desc* s, Plan& p) {
   if (!s) return refuse("scan: no description");
   if (s->T < 1 || s->N < 1 || s->D < 1 || s->G < 1) return refuse("scan: T, N, D and G must be positive");
   if (s->D % s->G) return refuse("scan: G must divide D");
@@ -432,28 +635,15 @@ int make_plan(const mjh_scan_desc* s, bool back, Plan& p) {
   a.dstate = s->dstate;
   a.T = s->T; a.N = s->N; a.D = s->D; a.G = s->G; a.K = s->D / s->G;
   p.heads = a.K > 1;
-  const int wide = s->dtype == MJH_F32 ? 2 : 4;
-  p.v = fits(*s, wide) ? wide : 1;
-  a.dv = a.D / p.v;
-  const ll threads = (ll)a.N * a.dv;
-  p.blocks = (unsigned)((threads + kBlock - 1) / kBlock);
-  const int per = (a.K + p.v - 1) / p.v;  // lanes a head needs
-  a.lanes = 1;
-  while (a.lanes < per && a.lanes < 64) a.lanes *= 2;
-  a.waves = (per + 63) / 64;
-  const ll slots = (ll)a.N * a.G;
-  const ll waves = a.waves == 1 ? (slots + 64 / a.lanes - 1) / (64 / a.lanes) : slots * a.waves;
-  p.head_blocks = (unsigned)((waves + 3) / 4);
+  set_width(p, fits(*s, kWide) ? kWide : 1);
   // chunks: enough threads to keep the card's loads in flight, each chunk some blocks of steps long
-  const ll want = 131072;
-  ll n = threads >= want ? 1 : (want + threads - 1) / threads;
+  const ll threads = (ll)a.N * a.dv;
   const ll blocks = (a.T + kSteps - 1) / kSteps;
-  n = std::max<ll>(1, std::min<ll>(n, blocks / 4));
-  n = std::min<ll>(n, 256);
+  ll n = threads >= kFull ? 1 : (kThreads + threads - 1) / threads;
+  n = std::max<ll>(1, std::min<ll>(std::min<ll>(n, blocks / kLeast), kMaxChunks));
   const ll per_chunk = (blocks + n - 1) / n;
   a.chunk = (int)(per_chunk * kSteps);
   a.nchunk = (int)((a.T + a.chunk - 1) / a.chunk);
-  (void)back;
   return 0;
 }
 
@@ -482,13 +672,18 @@ void launch_as(Kernel k, const Plan& p, hipStream_t s) {
   const dim3 grid(p.blocks, a.nchunk), block(kBlock);
   switch (k) {
     case kForward:
-      scan_forward<T, GT, V, GV, BLEND, false><<<grid, block, 0, s>>>(a);
+      if (a.nchunk > 1)
+        scan_forward<T, GT, V, GV, BLEND, false, true><<<grid, block, 0, s>>>(a);
+      else
+        scan_forward<T, GT, V, GV, BLEND, false, false><<<grid, block, 0, s>>>(a);
       break;
     case kForwardAgg:
-      scan_forward<T, GT, V, GV, BLEND, true><<<grid, block, 0, s>>>(a);
+      scan_forward<T, GT, V, GV, BLEND, true, true><<<grid, block, 0, s>>>(a);
+      scan_join<false><<<dim3((unsigned)(((ll)a.N * a.D + 63) / 64)), dim3(64 * ((a.nchunk + kJoin - 1) / kJoin)), 0, s>>>(a);
       break;
     case kBackwardAgg:
       scan_backward_agg<T, GT, V, GV, BLEND><<<grid, block, 0, s>>>(a);
+      scan_join<true><<<dim3((unsigned)(((ll)a.N * a.D + 63) / 64)), dim3(64 * ((a.nchunk + kJoin - 1) / kJoin)), 0, s>>>(a);
       break;
     case kBackward:
       if (!p.heads) {
@@ -506,16 +701,16 @@ void launch_as(Kernel k, const Plan& p, hipStream_t s) {
       break;
   }
 }
-template <class T, class GT, int WIDE>
+template <class T, class GT>
 void launch_typed(Kernel k, const Plan& p, int mode, hipStream_t s) {
   auto go = [&](auto blend) {
     constexpr bool B = decltype(blend)::value;
     if (p.v == 1)
       launch_as<T, GT, 1, 1, B>(k, p, s);
     else if (p.heads)
-      launch_as<T, GT, WIDE, 1, B>(k, p, s);
+      launch_as<T, GT, kWide, 1, B>(k, p, s);
     else
-      launch_as<T, GT, WIDE, WIDE, B>(k, p, s);
+      launch_as<T, GT, kWide, kWide, B>(k, p, s);
   };
   if (mode == MJH_SCAN_BLEND)
     go(std::true_type{});
@@ -526,11 +721,11 @@ int launch(Kernel k, const Plan& p, const mjh_scan_desc& d, void* stream) {
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const bool g32 = d.gtype == MJH_F32;
   if (d.dtype == MJH_F32)
-    launch_typed<float, float, 2>(k, p, d.mode, s);
+    launch_typed<float, float>(k, p, d.mode, s);
   else if (d.dtype == MJH_BF16)
-    g32 ? launch_typed<bf16, float, 4>(k, p, d.mode, s) : launch_typed<bf16, bf16, 4>(k, p, d.mode, s);
+    g32 ? launch_typed<bf16, float>(k, p, d.mode, s) : launch_typed<bf16, bf16>(k, p, d.mode, s);
   else
-    g32 ? launch_typed<f16, float, 4>(k, p, d.mode, s) : launch_typed<f16, f16, 4>(k, p, d.mode, s);
+    g32 ? launch_typed<f16, float>(k, p, d.mode, s) : launch_typed<f16, f16>(k, p, d.mode, s);
   return launched();
 }
 
@@ -547,13 +742,13 @@ int mjh_scan_steps(void) { return kSteps; }
 
 long long mjh_scan_workspace(const mjh_scan_desc* d, int back) {
   Plan p;
-  if (make_plan(d, back != 0, p)) return -1;
+  if (make_plan(d, p)) return -1;
   return 4 * (agg_floats(p) + (back ? part_floats(p) : 0));
 }
 
 int mjh_scan_forward(const mjh_scan_desc* d, void* stream) {
   Plan p;
-  if (int rc = make_plan(d, false, p)) return rc;
+  if (int rc = make_plan(d, p)) return rc;
   if (!d->x || !d->gate || !d->h || !d->last) return refuse("scan forward: x, gate, h and last are needed");
   if (d->ws_bytes < 4 * agg_floats(p) || (agg_floats(p) && !d->ws)) return refuse("scan forward: workspace too small");
   place(p, static_cast<float*>(d->ws));
@@ -564,7 +759,7 @@ int mjh_scan_forward(const mjh_scan_desc* d, void* stream) {
 
 int mjh_scan_backward(const mjh_scan_desc* d, void* stream) {
   Plan p;
-  if (int rc = make_plan(d, true, p)) return rc;
+  if (int rc = make_plan(d, p)) return rc;
   if (!d->x || !d->gate || !d->kept) return refuse("scan backward: x, gate and the kept states are needed");
   const ll need = agg_floats(p) + part_floats(p);
   if (d->ws_bytes < 4 * need || (need && !d->ws)) return refuse("scan backward: workspace too small");
@@ -576,7 +771,7 @@ int mjh_scan_backward(const mjh_scan_desc* d, void* stream) {
 
 int mjh_scan_step(const mjh_scan_desc* d, void* stream) {
   Plan p;
-  if (int rc = make_plan(d, false, p)) return rc;
+  if (int rc = make_plan(d, p)) return rc;
   if (d->T != 1) return refuse("scan step: T must be 1");
   if (!d->x || !d->gate || !d->h || !d->last || !d->state) return refuse("scan step: x, gate, state, h and last are needed");
   return launch(kStep, p, *d, stream);

@@ -76,6 +76,24 @@ __device__ __forceinline__ bool drop_keep(unsigned long long word, int odd, unsi
   return (unsigned long long)(odd ? (unsigned)word : (unsigned)(word >> 32)) >= thr;
 }
 
+// Neighbouring elements at any element's address: gfx950 takes 16-byte global accesses at any alignment, so a row
+// of an odd length is read as wide as an aligned one.
+template <class T, int V>
+struct __attribute__((packed, aligned(sizeof(T)))) Loose {
+  T v[V];
+};
+template <class T, int V>
+__device__ __forceinline__ Pack<T, V> load_loose(const T* p) {
+  return __builtin_bit_cast(Pack<T, V>, *reinterpret_cast<const Loose<T, V>*>(p));
+}
+template <class T, int V>
+__device__ __forceinline__ void store_loose(T* p, const float (&f)[V]) {
+  Pack<T, V> o;
+#pragma unroll
+  for (int k = 0; k < V; k++) o.v[k] = (T)f[k];
+  *reinterpret_cast<Loose<T, V>*>(p) = __builtin_bit_cast(Loose<T, V>, o);
+}
+
 inline bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
 }  // namespace mjh_seq

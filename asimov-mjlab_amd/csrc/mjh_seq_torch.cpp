@@ -492,8 +492,8 @@ struct Resnorm : torch::autograd::Function<Resnorm> {
     d.dys = d.drs = d.dgs = d.D;
     d.d_post_w = ptr(out[3]); d.d_post_b = ptr(out[4]); d.d_pre_w = ptr(out[5]); d.d_pre_b = ptr(out[6]); d.d_scale = ptr(out[7]);
     Tensor ws;
-    if (d.d_post_w || d.d_post_b || d.d_pre_w || d.d_pre_b || d.d_scale) {
-      d.ws_bytes = lib.resnorm_workspace(&d);
+    d.ws_bytes = lib.resnorm_workspace(&d);
+    if (d.ws_bytes != 0) {
       ws = workspace(d.ws_bytes, "mjh_resnorm_backward", a.r.t);
       d.ws = ptr(ws);
     }
