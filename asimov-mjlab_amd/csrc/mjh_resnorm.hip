@@ -6,13 +6,14 @@
 //   n = norm_pre(s)
 // The statistics, s inside n, and all sums are float32; s and n are rounded once, at their store.
 //
-// A group of lanes holds a row, 8 elements a lane, so every tensor is read once and every statistic is taken from
-// registers (the variance around the mean, in a second pass over registers). Rows of up to 512 elements: 8 to 64
-// lanes, several rows a workgroup, sums by lane exchanges; longer rows: a workgroup of as many waves as they need,
-// sums joined in shared memory. The backward pass keeps s and p nowhere: it forms them again from y, residual and
-// gate, the tensors that it has to read in any case, with the forward pass's (mean, rstd) of each row. The next
-// row's loads are under way while a row is worked on. Weight gradients: a group adds its rows in registers, groups
-// of a workgroup join in shared memory, workgroups in a second launch, each in a fixed order.
+// Rows of up to 2,048 elements (16-bit types: 4,096): a group of lanes holds a row, 8 elements a lane, so every tensor is read once and every
+// statistic is taken from registers (the variance around the mean, in a second pass over registers). 8 to 64 lanes,
+// several rows a workgroup, or a workgroup of two to eight waves. Longer rows: streams over the row, which read it
+// again, largely from the caches, where holding it would leave a CU one workgroup and nothing to hide its barriers.
+// The backward pass keeps s and p nowhere: it forms them again from y, residual and gate, the tensors that it has to
+// read in any case, with the forward pass's (mean, rstd) of each row. Weight gradients: a group (a thread that owns
+// columns) adds its rows in registers, groups of a workgroup join in shared memory, workgroups in a second launch,
+// each in a fixed order.
 #include <algorithm>
 #include <cstring>
 
@@ -21,9 +22,8 @@
 namespace {
 using namespace mjh_seq;
 
-constexpr int kPer = 8;     // elements a lane holds
-constexpr int kMaxDim = 1024 * kPer;
-constexpr ll kColumnWaves = 256 * 4 * 4;  // waves of the wide rows' column stream: 4 a SIMD
+constexpr int kPer = 8;  // elements a lane holds
+constexpr ll kColumnWaves = 256 * 4 * 4;  // waves of the long rows' column stream: 4 a SIMD
 constexpr int kSums = 5;    // post weight, post bias, scale, pre weight, pre bias
 enum { kPostW, kPostB, kScale, kPreW, kPreB };
 
@@ -43,13 +43,13 @@ struct Args {
   void* dr; ll drs;
   void* dgate; ll dgs;
   float* sums;    // (parts, kSums, D)
-  float* coef;    // (R, 4): the row sums of the wide rows' backward pass
+  float* coef;    // (R, 4): the row sums of the long rows' backward pass
   mjh_i64* ctr_out;
   Drop drop;
   float eps, inv;  // inv = 1 / D
   int R, D, layer, act, post, pre;
-  int tpr;    // lanes per row
-  int parts;  // workgroups (wide rows: row strands) of the backward pass
+  int tpr;    // lanes that hold a row
+  int parts;  // workgroups (long rows: strands of rows) of the backward pass
 };
 
 // The sum over groups of L neighbouring lanes, in every lane: four steps inside a row of 16 lanes (neighbours, pairs,
@@ -69,156 +69,75 @@ __device__ __forceinline__ float lane_sum(float v) {
   return v;
 }
 
-// FULL: the row fills its lanes, so there is no column to check.
-
-constexpr int threads_of(int tpr) { return tpr > 64 ? tpr : 256; }
-
-// TPR: 8 to 64 lanes hold a row; above, the most threads of a workgroup that holds one (a.tpr of them do).
-template <class T, bool FULL, int TPR>
-struct Row {
-  static constexpr int kVec = 16 / (int)sizeof(T);
-  static constexpr bool kWide = TPR > 64;
-  static constexpr int kThreads = threads_of(TPR);
-  static constexpr int kGroups = kWide ? 1 : 256 / TPR;  // rows a workgroup holds
-  static constexpr int kWaves = kThreads / 64;
-  int lane, group, lanes, D;
-  __device__ __forceinline__ explicit Row(const Args& a) : D(a.D) {
-    lanes = kWide ? a.tpr : TPR;
-    lane = kWide ? threadIdx.x : threadIdx.x % TPR;
-    group = kWide ? 0 : threadIdx.x / TPR;
+// Where a lane's N neighbouring elements of a row lie: slot p holds elements p N and on; what is left of a row that N
+// does not divide lies one element a slot behind them, so that no lane goes through a piece element by element.
+// FULL: every slot is a whole piece.
+template <class T, int N, bool FULL>
+struct Piece {
+  int c, cnt;  // first column; N, 1 or 0 columns
+  __device__ __forceinline__ Piece() {}
+  __device__ __forceinline__ Piece(int p, int D) {
+    const int whole = D / N, left = D - whole * N;
+    c = p < whole ? p * N : whole * N + (p - whole);
+    cnt = FULL || p < whole ? N : p < whole + left ? 1 : 0;
   }
-  // column of the lane's element k: pieces of kVec neighbours, the lanes' pieces side by side
-  __device__ __forceinline__ int col(int k) const { return (k / kVec * lanes + lane) * kVec + k % kVec; }
-  __device__ __forceinline__ bool has(int k) const { return FULL || col(k) < D; }
-  // elements k .. k + N of a lane, which are neighbours; the row may end among them
-  template <class W, int N>
-  __device__ __forceinline__ Pack<W, N> piece(const W* q, int k) const {
+  __device__ __forceinline__ bool has(int j) const { return FULL || j < cnt; }
+  template <class W>
+  __device__ __forceinline__ Pack<W, N> get(const W* q) const {
     Pack<W, N> v{};
-    if (FULL || col(k) + N <= D) {
-      v = load_loose<W, N>(q + col(k));
-    } else if (col(k) < D) {
-#pragma unroll
-      for (int j = 0; j < N; j++)
-        if (col(k + j) < D) v.v[j] = q[col(k + j)];
-    }
+    if (FULL || cnt == N)
+      v = load_loose<W, N>(q + c);
+    else if (cnt)
+      v.v[0] = q[c];
     return v;
   }
-  __device__ __forceinline__ void read(const void* p, ll row, ll step, bool on, T (&o)[kPer]) const {
-    const T* q = static_cast<const T*>(p) + row * step;
-#pragma unroll
-    for (int k = 0; k < kPer; k += kVec) {
-      Pack<T, kVec> v{};
-      if (on) v = piece<T, kVec>(q, k);
-#pragma unroll
-      for (int j = 0; j < kVec; j++) o[k + j] = v.v[j];
-    }
+  __device__ __forceinline__ Pack<T, N> read(const void* p, ll row, ll step) const {
+    return get(static_cast<const T*>(p) + row * step);
   }
-  __device__ __forceinline__ void write(void* p, ll row, ll step, bool on, const float (&f)[kPer]) const {
-    if (!on) return;
-    T* q = static_cast<T*>(p) + row * step;
-#pragma unroll
-    for (int k = 0; k < kPer; k += kVec) {
-      float o[kVec];
-#pragma unroll
-      for (int j = 0; j < kVec; j++) o[j] = f[k + j];
-      if (FULL || col(k) + kVec <= D) {
-        store_loose<T, kVec>(q + col(k), o);
-      } else if (col(k) < D) {
-#pragma unroll
-        for (int j = 0; j < kVec; j++)
-          if (col(k + j) < D) q[col(k + j)] = (T)o[j];
-      }
-    }
+  __device__ __forceinline__ void write(void* p, ll row, ll step, const float (&f)[N]) const {
+    T* q = static_cast<T*>(p) + row * step + c;
+    if (FULL || cnt == N)
+      store_loose<T, N>(q, f);
+    else if (cnt)
+      *q = (T)f[0];
   }
   // channel weights; `none` where there are none
-  template <class W>
-  __device__ __forceinline__ void weights_as(const void* w, float (&o)[kPer]) const {
-    constexpr int kBy = kVec * (int)sizeof(W) > 16 ? 16 / (int)sizeof(W) : kVec;
+  __device__ __forceinline__ void weights(const void* w, int w32, float none, float* o) const {
 #pragma unroll
-    for (int k = 0; k < kPer; k += kBy) {
-      const auto v = piece<W, kBy>(static_cast<const W*>(w), k);
+    for (int j = 0; j < N; j++) o[j] = none;
+    if (!w) return;
+    if (w32) {
+      const auto v = get(static_cast<const float*>(w));
 #pragma unroll
-      for (int j = 0; j < kBy; j++)
-        if (has(k + j)) o[k + j] = (float)v.v[j];
+      for (int j = 0; j < N; j++) o[j] = v.v[j];
+    } else {
+      const auto v = get(static_cast<const T*>(w));
+#pragma unroll
+      for (int j = 0; j < N; j++) o[j] = (float)v.v[j];
     }
   }
-  __device__ __forceinline__ void weights(const void* w, int w32, float none, float (&o)[kPer]) const {
-#pragma unroll
-    for (int k = 0; k < kPer; k++) o[k] = none;
-    if (w) w32 ? weights_as<float>(w, o) : weights_as<T>(w, o);
-  }
-  __device__ __forceinline__ void scales(const Args& a, float (&o)[kPer]) const {
+  __device__ __forceinline__ void scales(const Args& a, float* o) const {
     if (!a.scale_one) return weights(a.scale, a.w32, 1.f, o);
     const float one = a.w32 ? *static_cast<const float*>(a.scale) : (float)*static_cast<const T*>(a.scale);
 #pragma unroll
-    for (int k = 0; k < kPer; k++) o[k] = one;
+    for (int j = 0; j < N; j++) o[j] = one;
   }
-  // Sums of NV values over a row's lanes, in every lane. Wide rows: shared memory (kWaves * NV floats), two barriers.
-  template <int NV>
-  __device__ __forceinline__ void sum(float (&v)[NV], float* shared) const {
-#pragma unroll
-    for (int k = 0; k < NV; k++) v[k] = lane_sum<(kWide ? 64 : TPR)>(v[k]);
-    if constexpr (kWide) {
-      const int wave = threadIdx.x >> 6, waves = lanes >> 6;
-      if ((threadIdx.x & 63) == 0)
-#pragma unroll
-        for (int k = 0; k < NV; k++) shared[wave * NV + k] = v[k];
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < NV; k++) v[k] = 0.f;
-#pragma unroll
-      for (int j = 0; j < kWaves; j++)
-        if (j < waves)
-#pragma unroll
-          for (int k = 0; k < NV; k++) v[k] += shared[j * NV + k];
-      __syncthreads();
-    }
-  }
-  // mean and 1 / deviation of a row held in registers (columns beyond D hold 0 in v)
-  __device__ __forceinline__ void stats(const float (&v)[kPer], const Args& a, float* shared, float& mean, float& rstd) const {
-    mean = 0.f;
-    float t[1];
-    if (a.layer) {
-      t[0] = 0.f;
-#pragma unroll
-      for (int k = 0; k < kPer; k++) t[0] += v[k];
-      sum<1>(t, shared);
-      mean = t[0] * a.inv;
-    }
-    t[0] = 0.f;
-#pragma unroll
-    for (int k = 0; k < kPer; k++) {
-      const float c = has(k) ? v[k] - mean : 0.f;
-      t[0] += c * c;
-    }
-    sum<1>(t, shared);
-    rstd = __builtin_amdgcn_rsqf(__builtin_fmaf(t[0], a.inv, a.eps));  // to 1 ulp
-  }
-  // keep bits of the lane's elements (bit k: element k); the row's first element has index row * D. Neighbours
-  // share a word, and the words of a piece are one addition apart; in rows that begin at an odd index a piece
-  // begins with the second half of a word.
-  __device__ __forceinline__ unsigned keep_bits(unsigned long long base, const Drop& d, ll row) const {
+  // keep bits (bit j: element j). Neighbours share a word, and the words of a piece are one addition apart; a piece
+  // that begins at an odd index begins with the second half of a word.
+  __device__ __forceinline__ unsigned keep_bits(unsigned long long base, const Drop& d, ll row, int D) const {
+    const unsigned long long i = (unsigned long long)(row * D + c);
+    unsigned long long z = base + ((i >> 1) + 1ull) * 0x9e3779b97f4a7c15ull, w = mjh::mix64(z);
     unsigned bits = 0;
-    const bool odd = !FULL && (row * D & 1);
+    const bool odd = !FULL && (i & 1);
+    if (odd) bits = drop_keep(w, 1, d.thr);
 #pragma unroll
-    for (int k = 0; k < kPer; k += kVec) {
-      const unsigned long long i = (unsigned long long)(row * D + col(k));
-      unsigned long long z = base + ((i >> 1) + 1ull) * 0x9e3779b97f4a7c15ull, w = mjh::mix64(z);
-      if (odd) bits |= (unsigned)drop_keep(w, 1, d.thr) << k;
-#pragma unroll
-      for (int j = 0; j < kVec; j += 2) {
-        if (j > 0 || odd) {
-          z += 0x9e3779b97f4a7c15ull;
-          w = mjh::mix64(z);
-        }
-        const unsigned low = drop_keep(w, 0, d.thr), high = drop_keep(w, 1, d.thr);
-        if (odd) {
-          bits |= low << (k + j + 1);
-          if (j + 2 < kVec) bits |= high << (k + j + 2);
-        } else {
-          bits |= low << (k + j) | high << (k + j + 1);
-        }
+    for (int j = 0; j < N; j += 2) {
+      if (j > 0 || odd) {
+        z += 0x9e3779b97f4a7c15ull;
+        w = mjh::mix64(z);
       }
+      const unsigned low = drop_keep(w, 0, d.thr), high = drop_keep(w, 1, d.thr);
+      bits |= (low | high << 1) << (j + (odd ? 1 : 0));
     }
     return bits;
   }
@@ -267,63 +186,148 @@ __device__ __forceinline__ void activate(const T (&g)[N], const Args& a, float (
   }
 }
 
+// ---- rows held in registers -------------------------------------------------------------
+// TPR: 8 to 64 lanes hold a row; 256, 512: a workgroup of a.tpr threads (whole waves) does.
+constexpr int threads_of(int tpr) { return tpr > 256 ? tpr : 256; }
+template <class T, bool FULL, int TPR>
+struct Row {
+  static constexpr int N = 16 / (int)sizeof(T), kPieces = kPer / N;
+  static constexpr bool kWaves = TPR > 64;
+  static constexpr int kGroups = kWaves ? 1 : 256 / TPR;  // rows a workgroup holds
+  int group, lane, lanes, D, turn = 0;
+  Piece<T, N, FULL> at[kPieces];
+  __device__ __forceinline__ explicit Row(const Args& a) : D(a.D) {
+    lanes = kWaves ? a.tpr : TPR;
+    lane = kWaves ? threadIdx.x : threadIdx.x % TPR;
+    group = kWaves ? 0 : threadIdx.x / TPR;
+#pragma unroll
+    for (int k = 0; k < kPieces; k++) at[k] = Piece<T, N, FULL>(k * lanes + lane, a.D);
+  }
+  __device__ __forceinline__ bool has(int k) const { return at[k / N].has(k % N); }
+  __device__ __forceinline__ void read(const void* p, ll row, ll step, bool on, T (&o)[kPer]) const {
+#pragma unroll
+    for (int k = 0; k < kPieces; k++) {
+      Pack<T, N> v{};
+      if (on) v = at[k].read(p, row, step);
+#pragma unroll
+      for (int j = 0; j < N; j++) o[k * N + j] = v.v[j];
+    }
+  }
+  __device__ __forceinline__ void write(void* p, ll row, ll step, bool on, const float (&f)[kPer]) const {
+    if (!on) return;
+#pragma unroll
+    for (int k = 0; k < kPieces; k++) {
+      float o[N];
+#pragma unroll
+      for (int j = 0; j < N; j++) o[j] = f[k * N + j];
+      at[k].write(p, row, step, o);
+    }
+  }
+  __device__ __forceinline__ void weights(const void* w, int w32, float none, float (&o)[kPer]) const {
+#pragma unroll
+    for (int k = 0; k < kPieces; k++) at[k].weights(w, w32, none, o + k * N);
+  }
+  __device__ __forceinline__ void scales(const Args& a, float (&o)[kPer]) const {
+#pragma unroll
+    for (int k = 0; k < kPieces; k++) at[k].scales(a, o + k * N);
+  }
+  __device__ __forceinline__ unsigned keep_bits(unsigned long long base, const Drop& d, ll row) const {
+    unsigned bits = 0;
+#pragma unroll
+    for (int k = 0; k < kPieces; k++) bits |= (at[k].keep_bits(base, d, row, D) & ((1u << N) - 1u)) << (k * N);
+    return bits;
+  }
+  // Sums of NV values over a row's lanes, in every lane. Several waves: through shared memory (2 x 8 x 2 floats), in
+  // turns of two halves, so that one barrier keeps a turn's writes from the reads of the turn before the last.
+  template <int NV>
+  __device__ __forceinline__ void sum(float (&v)[NV], float (*shared)[16]) {
+#pragma unroll
+    for (int k = 0; k < NV; k++) v[k] = lane_sum<(kWaves ? 64 : TPR)>(v[k]);
+    if constexpr (kWaves) {
+      float* const s = shared[turn];
+      turn ^= 1;
+      if ((threadIdx.x & 63) == 0)
+#pragma unroll
+        for (int k = 0; k < NV; k++) s[(threadIdx.x >> 6) * 2 + k] = v[k];
+      __syncthreads();
+      const int waves = lanes >> 6;
+#pragma unroll
+      for (int k = 0; k < NV; k++) v[k] = s[k] + s[2 + k];
+#pragma unroll
+      for (int j = 2; j < TPR / 64; j++)
+        if (j < waves)
+#pragma unroll
+          for (int k = 0; k < NV; k++) v[k] += s[j * 2 + k];
+    }
+  }
+  // mean and 1 / deviation of a row held in registers (columns that are not there hold 0 in v)
+  __device__ __forceinline__ void stats(const float (&v)[kPer], const Args& a, float (*shared)[16], float& mean, float& rstd) {
+    mean = 0.f;
+    float t[1];
+    if (a.layer) {
+      t[0] = 0.f;
+#pragma unroll
+      for (int k = 0; k < kPer; k++) t[0] += v[k];
+      sum<1>(t, shared);
+      mean = t[0] * a.inv;
+    }
+    t[0] = 0.f;
+#pragma unroll
+    for (int k = 0; k < kPer; k++) {
+      const float c = has(k) ? v[k] - mean : 0.f;
+      t[0] += c * c;
+    }
+    sum<1>(t, shared);
+    rstd = __builtin_amdgcn_rsqf(__builtin_fmaf(t[0], a.inv, a.eps));  // to 1 ulp
+  }
+};
+
 template <class T, bool FULL, int TPR>
 __global__ __launch_bounds__(threads_of(TPR)) void resnorm_forward(const Args a) {
   typedef Row<T, FULL, TPR> R;
-  __shared__ float shared[R::kWaves];
-  const R at(a);
+  __shared__ float shared[2][16];
+  R at(a);
   if (a.ctr_out && blockIdx.x == 0 && threadIdx.x == 0) *a.ctr_out = a.drop.ctr ? *a.drop.ctr : 0;
   const bool block = a.y != nullptr;
   const unsigned long long base = a.drop.thr ? drop_base(a.drop) : 0;
-  // A workgroup of more than 256 threads takes the weights from the cache at every row and loads no row ahead: the
-  // registers buy a second workgroup on the CU instead.
-  constexpr bool kHold = R::kThreads <= 256;
   float post_w[kPer], post_b[kPer], pre_w[kPer], pre_b[kPer], scale[kPer];
-  if (kHold) {
-    at.weights(a.post_w, a.w32, 1.f, post_w);
-    at.weights(a.post_b, a.w32, 0.f, post_b);
-    at.weights(a.pre_w, a.w32, 1.f, pre_w);
-    at.weights(a.pre_b, a.w32, 0.f, pre_b);
-    at.scales(a, scale);
-  }
-  struct {
-    T r[kPer], y[kPer], g[kPer];
-  } cur, next;
-  auto fetch = [&](auto& to, ll row) {
+  at.weights(a.post_w, a.w32, 1.f, post_w);
+  at.weights(a.post_b, a.w32, 0.f, post_b);
+  at.weights(a.pre_w, a.w32, 1.f, pre_w);
+  at.weights(a.pre_b, a.w32, 0.f, pre_b);
+  at.scales(a, scale);
+  // No row is held while another is worked on: the waves that its registers cost hide more (65,536 x 300 bfloat16: 102 us against 125,
+  // 98,304 x 256: 56 against 57).
+  T raw[kPer], raw_y[kPer], raw_g[kPer];
+  auto fetch = [&](ll row) {
     const bool on = row < a.R;
-    at.read(a.r, row, a.rs, on, to.r);
-    if (block) at.read(a.y, row, a.ys, on, to.y);
-    if (a.gate) at.read(a.gate, row, a.gs, on, to.g);
+    at.read(a.r, row, a.rs, on, raw);
+    if (block) at.read(a.y, row, a.ys, on, raw_y);
+    if (a.gate) at.read(a.gate, row, a.gs, on, raw_g);
   };
   const ll step = (ll)gridDim.x * R::kGroups;
-  fetch(cur, (ll)blockIdx.x * R::kGroups + at.group);
+  fetch((ll)blockIdx.x * R::kGroups + at.group);
   for (ll first = (ll)blockIdx.x * R::kGroups; first < a.R; first += step) {
     const ll row = first + at.group;
     const bool on = row < a.R;
-    if (kHold) fetch(next, row + step);
-    float s[kPer], stats[4] = {0.f, 1.f, 0.f, 1.f};
+    float s[kPer], mean = 0.f, rstd = 1.f, pre_mean = 0.f, pre_rstd = 1.f;
 #pragma unroll
-    for (int k = 0; k < kPer; k++) s[k] = (float)cur.r[k];
+    for (int k = 0; k < kPer; k++) s[k] = (float)raw[k];
     if (block) {
       float p[kPer], av[kPer], slope[kPer];
 #pragma unroll
-      for (int k = 0; k < kPer; k++) p[k] = (float)cur.y[k];
+      for (int k = 0; k < kPer; k++) p[k] = (float)raw_y[k];
       if (a.post) {
-        at.stats(p, a, shared, stats[0], stats[1]);
-        if (!kHold) {
-          at.weights(a.post_w, a.w32, 1.f, post_w);
-          at.weights(a.post_b, a.w32, 0.f, post_b);
-        }
+        at.stats(p, a, shared, mean, rstd);
 #pragma unroll
-        for (int k = 0; k < kPer; k++) p[k] = __builtin_fmaf((p[k] - stats[0]) * stats[1], post_w[k], post_b[k]);
+        for (int k = 0; k < kPer; k++) p[k] = __builtin_fmaf((p[k] - mean) * rstd, post_w[k], post_b[k]);
       }
       if (a.drop.thr) {
         const unsigned keep = at.keep_bits(base, a.drop, row);
 #pragma unroll
         for (int k = 0; k < kPer; k++) p[k] = (keep >> k & 1u) ? p[k] * a.drop.scale : 0.f;
       }
-      activate<T, false>(cur.g, a, av, slope);
-      if (!kHold) at.scales(a, scale);
+      activate<T, false>(raw_g, a, av, slope);
 #pragma unroll
       for (int k = 0; k < kPer; k++) s[k] = __builtin_fmaf(scale[k], av[k] * p[k], s[k]);
       at.write(a.s, row, a.ss, on, s);
@@ -332,20 +336,13 @@ __global__ __launch_bounds__(threads_of(TPR)) void resnorm_forward(const Args a)
 #pragma unroll
       for (int k = 0; k < kPer; k++)
         if (!at.has(k)) s[k] = 0.f;
-      at.stats(s, a, shared, stats[2], stats[3]);
-      if (!kHold) {
-        at.weights(a.pre_w, a.w32, 1.f, pre_w);
-        at.weights(a.pre_b, a.w32, 0.f, pre_b);
-      }
+      at.stats(s, a, shared, pre_mean, pre_rstd);
 #pragma unroll
-      for (int k = 0; k < kPer; k++) s[k] = __builtin_fmaf((s[k] - stats[2]) * stats[3], pre_w[k], pre_b[k]);
+      for (int k = 0; k < kPer; k++) s[k] = __builtin_fmaf((s[k] - pre_mean) * pre_rstd, pre_w[k], pre_b[k]);
       at.write(a.n, row, a.ns, on, s);
     }
-    if (a.stats && on && at.lane == 0) store<float, 4>(a.stats + row * 4, stats);
-    if (kHold)
-      cur = next;
-    else
-      fetch(cur, row + step);
+    if (a.stats && on && at.lane == 0) store<float, 4>(a.stats + row * 4, {mean, rstd, pre_mean, pre_rstd});
+    fetch(row + step);
   }
 }
 
@@ -353,9 +350,9 @@ __global__ __launch_bounds__(threads_of(TPR)) void resnorm_forward(const Args a)
 template <class T, bool FULL, int TPR, bool BLOCK, bool BIAS>
 __global__ __launch_bounds__(threads_of(TPR)) void resnorm_backward(const Args a) {
   typedef Row<T, FULL, TPR> R;
-  __shared__ float shared[R::kWaves * 2];
+  __shared__ float shared[2][16];
   __shared__ float join[R::kGroups > 1 ? 256 * kPer : 1];
-  const R at(a);
+  R at(a);
   const unsigned long long base = BLOCK && a.drop.thr ? drop_base(a.drop) : 0;
   float post_w[kPer], post_b[kPer], pre_w[kPer], scale[kPer];
   at.weights(a.pre_w, a.w32, 1.f, pre_w);
@@ -369,31 +366,23 @@ __global__ __launch_bounds__(threads_of(TPR)) void resnorm_backward(const Args a
   for (int q = 0; q < kSums; q++)
 #pragma unroll
     for (int k = 0; k < kPer; k++) sum[q][k] = 0.f;
-  struct {
-    T r[kPer], y[kPer], g[kPer], ds[kPer], dn[kPer];
-    Pack<float, 4> st;
-  } cur, next;
-  auto fetch = [&](auto& to, ll row) {
-    const bool on = row < a.R;
-    to.st = Pack<float, 4>{};
-    if (on) to.st = load<float, 4>(a.stats + row * 4);
-    if (BLOCK) {
-      at.read(a.y, row, a.ys, on, to.y);
-      if (a.gate) at.read(a.gate, row, a.gs, on, to.g);
-    }
-    if (a.dn) {
-      at.read(a.r, row, a.rs, on, to.r);
-      at.read(a.dn, row, a.dns, on, to.dn);
-    }
-    if (a.ds) at.read(a.ds, row, a.dss, on, to.ds);
-  };
-  const ll step = (ll)gridDim.x * R::kGroups;
-  fetch(cur, (ll)blockIdx.x * R::kGroups + at.group);
-  for (ll first = (ll)blockIdx.x * R::kGroups; first < a.R; first += step) {
+  // No row is loaded ahead (98,304 x 256 bfloat16: 85 us against 108 with it).
+  for (ll first = (ll)blockIdx.x * R::kGroups; first < a.R; first += (ll)gridDim.x * R::kGroups) {
     const ll row = first + at.group;
     const bool on = row < a.R;
-    fetch(next, row + step);
-    const float mean = cur.st.v[0], rstd = cur.st.v[1], pre_mean = cur.st.v[2], pre_rstd = cur.st.v[3];
+    T raw_r[kPer], raw_y[kPer], raw_g[kPer], raw_ds[kPer], raw_dn[kPer];
+    Pack<float, 4> st{};
+    if (on) st = load<float, 4>(a.stats + row * 4);
+    if (BLOCK) {
+      at.read(a.y, row, a.ys, on, raw_y);
+      if (a.gate) at.read(a.gate, row, a.gs, on, raw_g);
+    }
+    if (a.dn) {
+      at.read(a.r, row, a.rs, on, raw_r);
+      at.read(a.dn, row, a.dns, on, raw_dn);
+    }
+    if (a.ds) at.read(a.ds, row, a.dss, on, raw_ds);
+    const float mean = st.v[0], rstd = st.v[1], pre_mean = st.v[2], pre_rstd = st.v[3];
     bool in[kPer];
 #pragma unroll
     for (int k = 0; k < kPer; k++) in[k] = on && at.has(k);
@@ -403,11 +392,11 @@ __global__ __launch_bounds__(threads_of(TPR)) void resnorm_backward(const Args a
     for (int k = 0; k < kPer; k++) ds[k] = 0.f;
     if (a.ds) {
 #pragma unroll
-      for (int k = 0; k < kPer; k++) ds[k] = (float)cur.ds[k];
+      for (int k = 0; k < kPer; k++) ds[k] = (float)raw_ds[k];
     }
     if (BLOCK) {
 #pragma unroll
-      for (int k = 0; k < kPer; k++) u[k] = yhat[k] = (float)cur.y[k];
+      for (int k = 0; k < kPer; k++) u[k] = yhat[k] = (float)raw_y[k];
       if (a.post) {
 #pragma unroll
         for (int k = 0; k < kPer; k++) {
@@ -420,16 +409,16 @@ __global__ __launch_bounds__(threads_of(TPR)) void resnorm_backward(const Args a
 #pragma unroll
         for (int k = 0; k < kPer; k++) u[k] = (keep >> k & 1u) ? u[k] * a.drop.scale : 0.f;
       }
-      activate<T, true>(cur.g, a, av, slope);
+      activate<T, true>(raw_g, a, av, slope);
     }
     if (a.dn) {
       float hat[kPer], t[2] = {0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < kPer; k++) {
-        const float r = (float)cur.r[k];
+        const float r = (float)raw_r[k];
         const float s = BLOCK ? __builtin_fmaf(scale[k], av[k] * u[k], r) : r;
         hat[k] = in[k] ? (s - pre_mean) * pre_rstd : 0.f;
-        const float dn = (float)cur.dn[k];
+        const float dn = (float)raw_dn[k];
         sum[kPreW][k] += dn * hat[k];
         if (BIAS) sum[kPreB][k] += dn;
         const float dv = in[k] ? dn * pre_w[k] : 0.f;
@@ -439,7 +428,7 @@ __global__ __launch_bounds__(threads_of(TPR)) void resnorm_backward(const Args a
       at.template sum<2>(t, shared);
       const float c0 = t[0] * a.inv, c1 = a.layer ? t[1] * a.inv : 0.f;
 #pragma unroll
-      for (int k = 0; k < kPer; k++) ds[k] += ((float)cur.dn[k] * pre_w[k] - hat[k] * c0 - c1) * pre_rstd;
+      for (int k = 0; k < kPer; k++) ds[k] += ((float)raw_dn[k] * pre_w[k] - hat[k] * c0 - c1) * pre_rstd;
     }
     if (a.dr) at.write(a.dr, row, a.drs, on, ds);
     if (BLOCK) {
@@ -472,7 +461,6 @@ __global__ __launch_bounds__(threads_of(TPR)) void resnorm_backward(const Args a
       }
       if (a.dy) at.write(a.dy, row, a.dys, on, ds);
     }
-    cur = next;
   }
   if (!a.sums) return;
   float* out = a.sums + (ll)blockIdx.x * kSums * a.D;
@@ -496,90 +484,188 @@ __global__ __launch_bounds__(threads_of(TPR)) void resnorm_backward(const Args a
     if (at.group == 0)
 #pragma unroll
       for (int k = 0; k < kPer; k++)
-        if (at.has(k)) out[q * a.D + at.col(k)] = sum[q][k];
+        if (at.has(k)) out[q * a.D + at.at[k / R::N].c + k % R::N] = sum[q][k];
   }
 }
 
-// ---- backward of rows longer than 2,048 elements ----
-// Held in registers, such a row with its weight sums leaves one workgroup a CU and nothing to hide its barriers
-// (2,047 x 4,097 floats: 170 us). Instead two streams: the first takes a row's sums, the second, whose threads own
-// columns and walk the rows, forms the gradients and the columns' sums. It reads the inputs again, largely from the
-// cache behind the L2.
+// ---- longer rows: streams over the row -------------------------------------------------------
+// Sum over a workgroup of 256 threads, in every thread; `shared` in turns of two halves as above.
+struct Block256 {
+  int turn = 0;
+  __device__ __forceinline__ float sum(float v, float (*shared)[4]) {
+    v = lane_sum<64>(v);
+    float* const s = shared[turn];
+    turn ^= 1;
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return (s[0] + s[1]) + (s[2] + s[3]);
+  }
+};
+
+// Mean and squared distance from it of the elements a thread has met, piece by piece (the pieces' own means are
+// merged, so a row far from 0 loses nothing), then over the workgroup around the row's mean. rms: plain squares.
+struct Moments {
+  float n = 0.f, mean = 0.f, m2 = 0.f;
+  template <int N>
+  __device__ __forceinline__ void add(const float (&v)[N], int cnt, int layer) {
+    if (!layer) {
+#pragma unroll
+      for (int j = 0; j < N; j++)
+        if (j < cnt) m2 += v[j] * v[j];
+      return;
+    }
+    if (!cnt) return;
+    const float k = (float)cnt, inv = cnt == N ? 1.f / N : 1.f;
+    float m = 0.f, q = 0.f;
+#pragma unroll
+    for (int j = 0; j < N; j++) m += j < cnt ? v[j] : 0.f;
+    m *= inv;
+#pragma unroll
+    for (int j = 0; j < N; j++) q += j < cnt ? (v[j] - m) * (v[j] - m) : 0.f;
+    const float share = k * __builtin_amdgcn_rcpf(n + k), d = m - mean;
+    m2 += q + d * d * n * share;
+    mean += d * share;
+    n += k;
+  }
+  __device__ __forceinline__ void finish(const Args& a, Block256& b, float (*shared)[4], float& row_mean, float& rstd) const {
+    row_mean = 0.f;
+    float t = m2;
+    if (a.layer) {
+      row_mean = b.sum(n * mean, shared) * a.inv;
+      t += n * (mean - row_mean) * (mean - row_mean);
+    }
+    rstd = __builtin_amdgcn_rsqf(__builtin_fmaf(b.sum(t, shared), a.inv, a.eps));
+  }
+};
+
+// One workgroup a row, three passes over it: the statistics of y; s, which is written, and its statistics; n. The
+// float32 s waits in shared memory for the last pass (KEEP, up to 8,192 columns, each thread's own), or is formed once
+// more: n is not taken from the rounded s.
+template <class T, bool KEEP>
+__global__ __launch_bounds__(256) void resnorm_stream(const Args a) {
+  constexpr int N = 16 / (int)sizeof(T);
+  __shared__ float shared[2][4];
+  extern __shared__ float kept[];  // slot by slot: (N, slots)
+  if (a.ctr_out && blockIdx.x == 0 && threadIdx.x == 0) *a.ctr_out = a.drop.ctr ? *a.drop.ctr : 0;
+  const ll row = blockIdx.x;
+  const bool block = a.y != nullptr;
+  const unsigned long long base = a.drop.thr ? drop_base(a.drop) : 0;
+  const int slots = a.D / N + a.D % N;
+  Block256 b;
+  float mean = 0.f, rstd = 1.f, pre_mean = 0.f, pre_rstd = 1.f;
+  if (block && a.post) {
+    Moments m;
+#pragma unroll 2
+    for (int p = threadIdx.x; p < slots; p += 256) {
+      const Piece<T, N, false> at(p, a.D);
+      const auto y = at.read(a.y, row, a.ys);
+      float v[N];
+#pragma unroll
+      for (int j = 0; j < N; j++) v[j] = (float)y.v[j];
+      m.add(v, at.cnt, a.layer);
+    }
+    m.finish(a, b, shared, mean, rstd);
+  }
+  auto form = [&](const Piece<T, N, false>& at, float (&s)[N]) {
+    const auto r = at.read(a.r, row, a.rs);
+#pragma unroll
+    for (int j = 0; j < N; j++) s[j] = (float)r.v[j];
+    if (!block) return;
+    const auto y = at.read(a.y, row, a.ys);
+    Pack<T, N> g{};
+    if (a.gate) g = at.read(a.gate, row, a.gs);
+    float p[N], av[N], slope[N], w[N], bias[N];
+#pragma unroll
+    for (int j = 0; j < N; j++) p[j] = (float)y.v[j];
+    if (a.post) {
+      at.weights(a.post_w, a.w32, 1.f, w);
+      at.weights(a.post_b, a.w32, 0.f, bias);
+#pragma unroll
+      for (int j = 0; j < N; j++) p[j] = __builtin_fmaf((p[j] - mean) * rstd, w[j], bias[j]);
+    }
+    if (a.drop.thr) {
+      const unsigned keep = at.keep_bits(base, a.drop, row, a.D);
+#pragma unroll
+      for (int j = 0; j < N; j++) p[j] = (keep >> j & 1u) ? p[j] * a.drop.scale : 0.f;
+    }
+    activate<T, false>(g.v, a, av, slope);
+    at.scales(a, w);
+#pragma unroll
+    for (int j = 0; j < N; j++) s[j] = __builtin_fmaf(w[j], av[j] * p[j], s[j]);
+  };
+  Moments m;
+  if (block || a.pre) {
+#pragma unroll 2
+    for (int p = threadIdx.x; p < slots; p += 256) {
+      const Piece<T, N, false> at(p, a.D);
+      float s[N];
+      form(at, s);
+      if (block) at.write(a.s, row, a.ss, s);
+      m.add(s, at.cnt, a.layer);
+      if (KEEP) {
+#pragma unroll
+        for (int j = 0; j < N; j++) kept[j * slots + p] = s[j];
+      }
+    }
+  }
+  if (a.pre) {
+    m.finish(a, b, shared, pre_mean, pre_rstd);
+#pragma unroll 2
+    for (int p = threadIdx.x; p < slots; p += 256) {
+      const Piece<T, N, false> at(p, a.D);
+      float s[N], w[N], bias[N];
+      if (KEEP) {
+#pragma unroll
+        for (int j = 0; j < N; j++) s[j] = kept[j * slots + p];
+      } else {
+        form(at, s);
+      }
+      at.weights(a.pre_w, a.w32, 1.f, w);
+      at.weights(a.pre_b, a.w32, 0.f, bias);
+#pragma unroll
+      for (int j = 0; j < N; j++) s[j] = __builtin_fmaf((s[j] - pre_mean) * pre_rstd, w[j], bias[j]);
+      at.write(a.n, row, a.ns, s);
+    }
+  }
+  if (a.stats && threadIdx.x == 0) store<float, 4>(a.stats + row * 4, {mean, rstd, pre_mean, pre_rstd});
+}
+
+// Backward, two streams: the first takes a row's sums, the second, whose threads own columns and walk the rows, forms
+// the gradients and the columns' sums (held in registers instead, 2,047 x 4,097 floats took 170 us, these 100).
 //
 // The norm of y needs sums over ds, the gradient of s, which itself has the row's sums c0, c1 in it. It is linear
 // in them, ds = X - rstd (hat c0 + c1) with X = ds_in + rstd dn w, so the first stream takes the sums of X q, hat q
 // and q (q = the factor from ds to the gradient of the normalised y, once times yhat, once alone) in the same pass.
+// 4 elements a thread, whatever the type: 8 of a 16-bit type cost the registers of half the waves (2,048 x 8,192
+// bfloat16: 104 us against 72).
+constexpr int kBack = 4;
 template <class T>
-struct Piece {
-  static constexpr int N = 16 / (int)sizeof(T);
-  int c, D;
-  template <class W, int M>
-  __device__ __forceinline__ Pack<W, M> get(const W* q, int at) const {
-    Pack<W, M> v{};
-    if (at + M <= D) {
-      v = load_loose<W, M>(q + at);
-    } else if (at < D) {
-#pragma unroll
-      for (int j = 0; j < M; j++)
-        if (at + j < D) v.v[j] = q[at + j];
+using BackPiece = Piece<T, kBack, false>;
+
+template <class T>
+struct Raw {
+  Pack<T, kBack> y, r, g, ds, dn;
+  template <bool BLOCK>
+  __device__ __forceinline__ void fetch(const Args& a, const BackPiece<T>& at, ll row) {
+    if (BLOCK) {
+      y = at.read(a.y, row, a.ys);
+      if (a.gate) g = at.read(a.gate, row, a.gs);
     }
-    return v;
-  }
-  __device__ __forceinline__ Pack<T, N> read(const void* p, ll row, ll step) const {
-    return get<T, N>(static_cast<const T*>(p) + row * step, c);
-  }
-  __device__ __forceinline__ void write(void* p, ll row, ll step, const float (&f)[N]) const {
-    T* q = static_cast<T*>(p) + row * step + c;
-    if (c + N <= D) {
-      store_loose<T, N>(q, f);
-    } else {
-#pragma unroll
-      for (int j = 0; j < N; j++)
-        if (c + j < D) q[j] = (T)f[j];
+    if (a.dn) {
+      r = at.read(a.r, row, a.rs);
+      dn = at.read(a.dn, row, a.dns);
     }
-  }
-  __device__ __forceinline__ void weights(const void* w, int w32, float none, float (&o)[N]) const {
-#pragma unroll
-    for (int j = 0; j < N; j++) o[j] = none;
-    if (!w) return;
-    if (w32) {
-#pragma unroll
-      for (int k = 0; k < N; k += 4) {
-        const auto v = get<float, 4>(static_cast<const float*>(w), c + k);
-#pragma unroll
-        for (int j = 0; j < 4; j++) o[k + j] = v.v[j];
-      }
-    } else {
-      const auto v = get<T, N>(static_cast<const T*>(w), c);
-#pragma unroll
-      for (int j = 0; j < N; j++) o[j] = (float)v.v[j];
-    }
-  }
-  __device__ __forceinline__ void scales(const Args& a, float (&o)[N]) const {
-    if (!a.scale_one) return weights(a.scale, a.w32, 1.f, o);
-    const float one = a.w32 ? *static_cast<const float*>(a.scale) : (float)*static_cast<const T*>(a.scale);
-#pragma unroll
-    for (int j = 0; j < N; j++) o[j] = one;
-  }
-  __device__ __forceinline__ unsigned keep_bits(unsigned long long base, const Drop& d, ll row) const {
-    unsigned bits = 0;
-#pragma unroll
-    for (int j = 0; j < N; j++) {
-      const unsigned long long i = (unsigned long long)(row * D + c + j);
-      bits |= (unsigned)drop_keep(drop_word(base, i >> 1), (int)(i & 1), d.thr) << j;
-    }
-    return bits;
+    if (a.ds) ds = at.read(a.ds, row, a.dss);
   }
 };
 
 // What both streams form of a row's piece before its sums are known.
 template <class T, bool BLOCK, bool BIAS>
 struct Formed {
-  static constexpr int N = Piece<T>::N;
+  static constexpr int N = kBack;
   float ds[N], dn[N], hat[N], yhat[N], u[N], av[N], slope[N];
   unsigned keep;
-  template <class Raw>
-  __device__ __forceinline__ Formed(const Args& a, const Piece<T>& at, const Raw& raw, const Pack<float, 4>& st, ll row,
+  __device__ __forceinline__ Formed(const Args& a, const BackPiece<T>& at, const Raw<T>& raw, const Pack<float, 4>& st, ll row,
                                     unsigned long long base, const float (&post_w)[N], const float (&post_b)[N],
                                     const float (&scale)[N]) {
     keep = ~0u;
@@ -597,7 +683,7 @@ struct Formed {
         u[j] = a.post ? (BIAS ? __builtin_fmaf(yhat[j], post_w[j], post_b[j]) : yhat[j] * post_w[j]) : yhat[j];
       }
       if (a.drop.thr) {
-        keep = at.keep_bits(base, a.drop, row);
+        keep = at.keep_bits(base, a.drop, row, a.D);
 #pragma unroll
         for (int j = 0; j < N; j++) u[j] = (keep >> j & 1u) ? u[j] * a.drop.scale : 0.f;
       }
@@ -607,39 +693,24 @@ struct Formed {
 #pragma unroll
       for (int j = 0; j < N; j++) {
         const float s = BLOCK ? __builtin_fmaf(scale[j], av[j] * u[j], hat[j]) : hat[j];
-        hat[j] = at.c + j < a.D ? (s - st.v[2]) * st.v[3] : 0.f;
+        hat[j] = at.has(j) ? (s - st.v[2]) * st.v[3] : 0.f;
       }
     }
-  }
-};
-template <class T>
-struct Raw {
-  Pack<T, Piece<T>::N> y, r, g, ds, dn;
-  template <bool BLOCK>
-  __device__ __forceinline__ void fetch(const Args& a, const Piece<T>& at, ll row) {
-    if (BLOCK) {
-      y = at.read(a.y, row, a.ys);
-      if (a.gate) g = at.read(a.gate, row, a.gs);
-    }
-    if (a.dn) {
-      r = at.read(a.r, row, a.rs);
-      dn = at.read(a.dn, row, a.dns);
-    }
-    if (a.ds) ds = at.read(a.ds, row, a.dss);
   }
 };
 
 // One workgroup a row: (c0, c1) of the norm before, (c0, c1) of the norm of y.
 template <class T, bool BLOCK, bool BIAS>
 __global__ __launch_bounds__(256) void resnorm_rows(const Args a) {
-  constexpr int N = Piece<T>::N;
+  constexpr int N = kBack;
   __shared__ float shared[4][8];
   const ll row = blockIdx.x;
   const unsigned long long base = BLOCK && a.drop.thr ? drop_base(a.drop) : 0;
   const auto st = load<float, 4>(a.stats + row * 4);
+  const int slots = a.D / N + a.D % N;
   float t[8] = {};  // dv hat, dv, X q0, hat q0, q0, X q1, hat q1, q1
-  for (int c = threadIdx.x * N; c < a.D; c += 256 * N) {
-    const Piece<T> at{c, a.D};
+  for (int p = threadIdx.x; p < slots; p += 256) {
+    const BackPiece<T> at(p, a.D);
     Raw<T> raw;
     raw.template fetch<BLOCK>(a, at, row);
     float pre_w[N], post_w[N], post_b[N], scale[N];
@@ -652,7 +723,7 @@ __global__ __launch_bounds__(256) void resnorm_rows(const Args a) {
     const Formed<T, BLOCK, BIAS> f(a, at, raw, st, row, base, post_w, post_b, scale);
 #pragma unroll
     for (int j = 0; j < N; j++) {
-      if (c + j >= a.D) continue;
+      if (!at.has(j)) continue;
       const float dv = f.dn[j] * pre_w[j];
       t[0] += dv * f.hat[j];
       t[1] += dv;
@@ -685,12 +756,12 @@ __global__ __launch_bounds__(256) void resnorm_rows(const Args a) {
   store<float, 4>(a.coef + row * 4, out);
 }
 
-// A wave owns 64 pieces of columns and walks rows blockIdx.y, + gridDim.y, ...
+// A wave owns 64 slots of columns and walks rows blockIdx.y, + gridDim.y, ...
 template <class T, bool BLOCK, bool BIAS>
 __global__ __launch_bounds__(64) void resnorm_columns(const Args a) {
-  constexpr int N = Piece<T>::N;
-  const Piece<T> at{(int)(blockIdx.x * 64 + threadIdx.x) * N, a.D};
-  if (at.c >= a.D) return;
+  constexpr int N = kBack;
+  const BackPiece<T> at(blockIdx.x * 64 + threadIdx.x, a.D);
+  if (!at.cnt) return;
   const unsigned long long base = BLOCK && a.drop.thr ? drop_base(a.drop) : 0;
   float pre_w[N], post_w[N], post_b[N], scale[N];
   at.weights(a.pre_w, a.w32, 1.f, pre_w);
@@ -747,7 +818,7 @@ __global__ __launch_bounds__(64) void resnorm_columns(const Args a) {
     if (!BIAS && (q == kPostB || q == kPreB)) continue;
 #pragma unroll
     for (int j = 0; j < N; j++)
-      if (at.c + j < a.D) out[q * a.D + at.c + j] = sum[q][j];
+      if (at.has(j)) out[q * a.D + at.c + j] = sum[q][j];
   }
 }
 
@@ -859,22 +930,23 @@ __global__ __launch_bounds__(256) void dropout_rows(const DropArgs a) {
 }
 
 // ---- host side ------------------------------------------------------------------------
-// lanes that hold a row, and the workgroup that does: whole waves beyond one
-int lanes_of(int D) {
-  if (D > 64 * kPer) return (D + 64 * kPer - 1) / (64 * kPer) * 64;
+// lanes that hold a row (8 elements each, as slots of 16 bytes): a power of two up to a wave, then whole waves
+int lanes_of(int D, int dtype) {
+  const int n = dtype == MJH_F32 ? 4 : 8, slots = D / n + D % n, lanes = (slots * n + kPer - 1) / kPer;
+  if (lanes > 64) return (lanes + 63) / 64 * 64;
   int t = 8;
-  while (t * kPer < D) t *= 2;
+  while (t < lanes) t *= 2;
   return t;
 }
+bool long_row(int D, int dtype) { return lanes_of(D, dtype) > (dtype == MJH_F32 ? 256 : 512); }
 
 // the backward pass's parts write partial sums each, so a part takes several rows
-bool wide(int D) { return D > 256 * kPer; }
 unsigned parts_of(int D, ll rows, int dtype) {
-  const int lanes = lanes_of(D);
-  if (wide(D)) {
-    const ll tiles = (D + 64 * (dtype == MJH_F32 ? 4 : 8) - 1) / (64 * (dtype == MJH_F32 ? 4 : 8));
+  if (long_row(D, dtype)) {
+    const ll tiles = (D / kBack + D % kBack + 63) / 64;
     return (unsigned)std::max<ll>(1, std::min<ll>(rows / 4, kColumnWaves / tiles));
   }
+  const int lanes = lanes_of(D, dtype);
   const ll groups = lanes > 64 ? 1 : 256 / lanes, waves = lanes > 64 ? lanes / 64 : 4;
   return (unsigned)std::max<ll>(1, std::min<ll>((rows + groups - 1) / groups / 4, 256 * 12 / waves));
 }
@@ -882,9 +954,9 @@ unsigned parts_of(int D, ll rows, int dtype) {
 int check(const mjh_resnorm_desc* d) {
   if (!d) return refuse("residual norm: no description");
   if (d->R < 1 || d->D < 1) return refuse("residual norm: R and D must be positive");
-  if (d->D > kMaxDim) return refuse("residual norm: D is at most 8192");
   if (d->R > 0x7fffffffll) return refuse("residual norm: R must be below 2^31");
   if (d->dtype < 0 || d->dtype > 2) return refuse("residual norm: unknown type");
+  if (d->D > 1 << 24) return refuse("residual norm: D is at most 2^24");
   if (!d->r) return refuse("residual norm: the residual is needed");
   if (!d->y && (d->gate || d->post || d->scale)) return refuse("residual norm: gate, post norm and scale need y");
   if (d->thr > (1ull << 32)) return refuse("dropout: threshold above 2^32");
@@ -913,44 +985,31 @@ Args args_of(const mjh_resnorm_desc& d) {
   a.eps = d.eps;
   a.inv = (float)(1.0 / d.D);
   a.R = (int)d.R; a.D = d.D; a.layer = d.layer; a.act = d.act; a.post = d.post; a.pre = d.pre;
-  a.tpr = lanes_of(d.D);
+  a.tpr = lanes_of(d.D, d.dtype);
   a.parts = (int)parts_of(d.D, d.R, d.dtype);
   return a;
 }
 
-// rows of which a workgroup (a wave of the wide rows' column stream) takes one after another
-unsigned grid_of(int lanes, ll rows) {
-  const int groups = lanes > 64 ? 1 : 256 / lanes;
-  const ll need = (rows + groups - 1) / groups;
-  return (unsigned)std::min<ll>(need, 256 * 32 / (lanes > 64 ? lanes / 64 : 4));
-}
 bool wants_bias(const mjh_resnorm_desc& d) { return d.post_b || d.pre_b; }
 
 template <class T, bool FULL, int TPR>
 void launch_forward(const Args& a, hipStream_t s) {
-  resnorm_forward<T, FULL, TPR><<<dim3(grid_of(a.tpr, a.R)), dim3(TPR > 64 ? a.tpr : 256), 0, s>>>(a);
+  const ll groups = TPR > 64 ? 1 : 256 / TPR, waves = TPR > 64 ? a.tpr / 64 : 4;
+  const ll need = (a.R + groups - 1) / groups;
+  resnorm_forward<T, FULL, TPR><<<dim3((unsigned)std::min<ll>(need, 256 * 32 / waves)), dim3(TPR > 64 ? a.tpr : 256), 0, s>>>(a);
 }
 template <class T, bool FULL, int TPR, bool BLOCK, bool BIAS>
 void launch_backward(const Args& a, hipStream_t s) {
   resnorm_backward<T, FULL, TPR, BLOCK, BIAS><<<dim3(a.parts), dim3(TPR > 64 ? a.tpr : 256), 0, s>>>(a);
 }
-template <class T, bool BLOCK, bool BIAS>
-void launch_wide(const Args& a, hipStream_t s) {
-  constexpr int N = 64 * Piece<T>::N;
-  resnorm_rows<T, BLOCK, BIAS><<<dim3(a.R), dim3(256), 0, s>>>(a);
-  resnorm_columns<T, BLOCK, BIAS><<<dim3((a.D + N - 1) / N, a.parts), dim3(64), 0, s>>>(a);
-}
 template <class T, bool FULL>
 void launch_forward_rows(const Args& a, hipStream_t s) {
-  // the fewest threads a workgroup is compiled for leave a lane the most registers
   if (a.tpr == 8) return launch_forward<T, FULL, 8>(a, s);
   if (a.tpr == 16) return launch_forward<T, FULL, 16>(a, s);
   if (a.tpr == 32) return launch_forward<T, FULL, 32>(a, s);
   if (a.tpr == 64) return launch_forward<T, FULL, 64>(a, s);
-  if (a.tpr <= 256) return launch_forward<T, FULL, 256>(a, s);
-  if (a.tpr <= 512) return launch_forward<T, FULL, 512>(a, s);
-  if (a.tpr <= 768) return launch_forward<T, FULL, 768>(a, s);
-  launch_forward<T, FULL, 1024>(a, s);
+  if (sizeof(T) == 4 || a.tpr <= 256) return launch_forward<T, FULL, 256>(a, s);
+  if constexpr (sizeof(T) == 2) launch_forward<T, FULL, 512>(a, s);
 }
 template <class T, bool FULL, bool BLOCK, bool BIAS>
 void launch_backward_rows(const Args& a, hipStream_t s) {
@@ -958,20 +1017,33 @@ void launch_backward_rows(const Args& a, hipStream_t s) {
   if (a.tpr == 16) return launch_backward<T, FULL, 16, BLOCK, BIAS>(a, s);
   if (a.tpr == 32) return launch_backward<T, FULL, 32, BLOCK, BIAS>(a, s);
   if (a.tpr == 64) return launch_backward<T, FULL, 64, BLOCK, BIAS>(a, s);
-  launch_backward<T, FULL, 256, BLOCK, BIAS>(a, s);
+  if (sizeof(T) == 4 || a.tpr <= 256) return launch_backward<T, FULL, 256, BLOCK, BIAS>(a, s);
+  if constexpr (sizeof(T) == 2) launch_backward<T, FULL, 512, BLOCK, BIAS>(a, s);
 }
 template <class T, bool BLOCK, bool BIAS>
-void launch_backward_as(const Args& a, hipStream_t s) {
-  if (wide(a.D)) return launch_wide<T, BLOCK, BIAS>(a, s);
-  a.tpr * kPer == a.D ? launch_backward_rows<T, true, BLOCK, BIAS>(a, s) : launch_backward_rows<T, false, BLOCK, BIAS>(a, s);
+void launch_backward_as(const Args& a, bool streams, hipStream_t s) {
+  if (streams) {
+    resnorm_rows<T, BLOCK, BIAS><<<dim3(a.R), dim3(256), 0, s>>>(a);
+    resnorm_columns<T, BLOCK, BIAS><<<dim3((a.D / kBack + a.D % kBack + 63) / 64, a.parts), dim3(64), 0, s>>>(a);
+  } else if (a.tpr * kPer == a.D) {
+    launch_backward_rows<T, true, BLOCK, BIAS>(a, s);
+  } else {
+    launch_backward_rows<T, false, BLOCK, BIAS>(a, s);
+  }
 }
 template <class T>
 void launch_type(const mjh_resnorm_desc& d, const Args& a, bool back, hipStream_t s) {
-  if (!back) return a.tpr * kPer == a.D ? launch_forward_rows<T, true>(a, s) : launch_forward_rows<T, false>(a, s);
-  if (a.y)
-    wants_bias(d) ? launch_backward_as<T, true, true>(a, s) : launch_backward_as<T, true, false>(a, s);
+  const bool streams = long_row(d.D, d.dtype), bias = wants_bias(d);
+  if (back && a.y)
+    bias ? launch_backward_as<T, true, true>(a, streams, s) : launch_backward_as<T, true, false>(a, streams, s);
+  else if (back)
+    bias ? launch_backward_as<T, false, true>(a, streams, s) : launch_backward_as<T, false, false>(a, streams, s);
+  else if (streams && a.D <= 8192)
+    resnorm_stream<T, true><<<dim3(a.R), dim3(256), 4 * (16 / sizeof(T)) * (a.D / (16 / sizeof(T)) + a.D % (16 / sizeof(T))), s>>>(a);
+  else if (streams)
+    resnorm_stream<T, false><<<dim3(a.R), dim3(256), 0, s>>>(a);
   else
-    wants_bias(d) ? launch_backward_as<T, false, true>(a, s) : launch_backward_as<T, false, false>(a, s);
+    a.tpr * kPer == a.D ? launch_forward_rows<T, true>(a, s) : launch_forward_rows<T, false>(a, s);
 }
 void launch(const mjh_resnorm_desc& d, const Args& a, bool back, hipStream_t s) {
   if (d.dtype == MJH_F32)
@@ -1004,8 +1076,8 @@ extern "C" {
 
 long long mjh_resnorm_workspace(const mjh_resnorm_desc* d) {
   if (check(d)) return -1;
-  // partial sums, the scale's column sums, the row sums of wide rows (first: 16-byte aligned)
-  return 4 * ((wide(d->D) ? 4 * d->R : 0) + (ll)parts_of(d->D, d->R, d->dtype) * kSums * d->D + d->D);
+  // row sums of long rows (first: 16-byte aligned), partial sums, the scale's column sums
+  return 4 * ((long_row(d->D, d->dtype) ? 4 * d->R : 0) + (ll)parts_of(d->D, d->R, d->dtype) * kSums * d->D + d->D);
 }
 
 int mjh_resnorm_forward(const mjh_resnorm_desc* d, void* stream) {
@@ -1019,12 +1091,12 @@ int mjh_resnorm_backward(const mjh_resnorm_desc* d, void* stream) {
   if (int rc = check(d)) return rc;
   if (!d->stats || (!d->ds && !d->dn) || (d->dn && !d->pre)) return refuse("residual norm backward: statistics or gradients are missing");
   const bool sums = d->d_post_w || d->d_post_b || d->d_scale || d->d_pre_w || d->d_pre_b;
-  if ((sums || wide(d->D)) && (!d->ws || d->ws_bytes < mjh_resnorm_workspace(d)))
+  if ((sums || long_row(d->D, d->dtype)) && (!d->ws || d->ws_bytes < mjh_resnorm_workspace(d)))
     return refuse("residual norm backward: workspace too small");
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   Args a = args_of(*d);
   a.coef = static_cast<float*>(d->ws);
-  a.sums = sums ? static_cast<float*>(d->ws) + (wide(a.D) ? 4 * (ll)a.R : 0) : nullptr;
+  a.sums = sums ? static_cast<float*>(d->ws) + (long_row(d->D, d->dtype) ? 4 * (ll)a.R : 0) : nullptr;
   launch(*d, a, true, s);
   if (int rc = launched()) return rc;
   if (!sums) return 0;

@@ -539,7 +539,7 @@ py::object residual_norm(const Maybe& y_, const Tensor& r, const Maybe& pre_w_,
   Norm o{norm, act, eps, p, check_drop(name, p, seed, key, ctr, r)};
   if (!y.defined()) o.r.thr = 0;
   if (!r.is_cuda() || r.numel() == 0) return py::none();
-  if (dim > 8192) refuse(name, ": rows of at most 8192 elements, got ", dim);
+  if (dim > 1 << 24 || r.numel() / dim > 0x7fffffff) refuse(name, ": at most 2^31 rows of at most 2^24 elements, got ", r.sizes());
   Tensor s = r, n;
   if (wants_grad({&y, &r, &gate, &w[0], &w[1], &w[2], &w[3], &w[4]})) {
     auto out = Resnorm::apply(maybe(y), maybe(r), maybe(gate), maybe(w[0]), maybe(w[1]), maybe(w[2]), maybe(w[3]), maybe(w[4]), maybe(ctr),

@@ -185,7 +185,7 @@ def residual_norm(y: torch.Tensor | None, residual: torch.Tensor, *, pre_weight:
 
   ``s = residual + scale * act(gate) * dropout(norm(y))`` and ``n = norm(s)``
 
-  y, residual and gate are (..., D) of one type, D at most 8192. ``post_weight`` (D,) turns the norm of y
+  y, residual and gate are (..., D) of one type, D at most 2^24. ``post_weight`` (D,) turns the norm of y
   on, ``pre_weight`` (D,) the norm of s (else n is None); ``post_bias`` / ``pre_bias`` add to them. ``norm``
   is "rms" (x / sqrt(mean x^2 + eps) * weight) or "layer" (around the mean). ``act`` is "silu" or
   "sigmoid"; no gate: 1. ``scale`` is a tensor of D elements, or of one; None: 1. Dropout as in

@@ -690,7 +690,7 @@ int mjh_scan_backward(const mjh_scan_desc* d, void* stream);
 /* T = 1 for serving: last = the state after the step (may be state itself). */
 int mjh_scan_step(const mjh_scan_desc* d, void* stream);
 
-/* R rows of D <= 8192 columns at row strides *s:
+/* R rows of D <= 2^24 columns at row strides *s:
  *   p = norm(y) (post != 0: rms or, layer != 0, layer norm with post_w / post_b), or y
  *   u = dropout(p) (thr = round(prob 2^32); 0 = none; element index row * D + column)
  *   s = r + scale * act(gate) * u       n = norm(s) (pre != 0, pre_w / pre_b)

@@ -257,7 +257,7 @@ def check_norm(v, ds, dn, norm="rms", act="silu", p=0.0, seed=3, key=4, ctr=None
 @pytest.mark.parametrize("norm", ["rms", "layer"])
 @pytest.mark.parametrize("dtype,wtype", [(F32, F32), (BF16, F32), (BF16, BF16), (F16, F16)])
 @pytest.mark.parametrize("r,d", [(1, 1), (3, 2), (5, 64), (33, 99), (70, 128), (9, 256), (40, 512), (7, 1000), (5, 1024),
-                                 (11, 2048), (3, 2050), (4, 4096), (9, 4097), (2, 8192), (3, 8191)])
+                                 (11, 2048), (3, 2050), (4, 4096), (9, 4097), (2, 8192), (3, 8191), (37, 2047), (2, 20001), (5, 300), (6, 515)])
 def test_residual_norm(r, d, dtype, wtype, norm):
   v, ds, dn = norm_inputs(r, d, dtype, wtype, bias=norm == "layer", scaled=1 if d % 2 == 0 else 2)
   check_norm(v, ds, dn, norm, act="silu" if d % 3 else "sigmoid", p=0.3 if r % 2 else 0.0,
@@ -461,8 +461,8 @@ def test_gpu_refusals():
   x = rnd(4, 2, 8)
   with pytest.raises(ValueError, match="is on"):
     seqops.gated_scan(x, x, torch.zeros(2, 8))
-  with pytest.raises(ValueError, match="at most 8192"):
-    seqops.residual_norm(None, torch.zeros(2, 8200, device="cuda"), pre_weight=torch.ones(8200, device="cuda"))
+  with pytest.raises(ValueError, match="2.24 elements"):
+    seqops.residual_norm(None, torch.zeros(1, (1 << 24) + 1, device="cuda"), pre_weight=torch.ones((1 << 24) + 1, device="cuda"))
   with pytest.raises(ValueError, match="ctr must be"):
     seqops.dropout(x, 0.5, 1, 0, torch.zeros(1, dtype=torch.int64))
   leaf = x.detach().requires_grad_()

@@ -235,7 +235,7 @@ def test_entry_points_refuse_before_any_launch():
   assert lib.mjh_scan_workspace(ctypes.byref(_scan_desc(G=4)), 1) == -1
   r = seq_ref.ResnormDesc()
   r.R, r.D, r.pre = 2, 9000, 1
-  for kw, why in ((dict(), b"8192"), (dict(D=8), b"residual is needed"), (dict(D=8, r=1024, gate=1024), b"need y"),
+  for kw, why in ((dict(D=(1 << 24) + 1), b"2^24"), (dict(D=8), b"residual is needed"), (dict(D=8, r=1024, gate=1024), b"need y"),
                   (dict(D=8, r=1024, n=None), b"output"), (dict(D=8, r=1024, n=1024, thr=1 << 33), b"threshold")):
     for k in ("gate", "r", "n"):
       setattr(r, k, None)
