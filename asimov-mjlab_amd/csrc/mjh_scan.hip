@@ -116,17 +116,17 @@ struct Gate {
 };
 
 // The chunks' results become the state that comes into each chunk (forward: from the chunks before it; BACK: the
-// gradient from the chunks after it), written over the chunk's own result in agg_b. A workgroup holds 64 channels
-// by 16 waves; a wave takes kJoin neighbouring chunks, all loads in flight at once (one thread a channel and a loop
-// over 256 chunks took 70 us, this 5). A chunk with a reset inside passes nothing on, whatever comes in (not 0 times
-// it: the state before a reset may be infinite or NaN).
-constexpr int kJoin = 16, kMaxChunks = 16 * kJoin;
+// gradient from the chunks after it), written over the chunk's own result in agg_b. A workgroup holds 32 channels
+// by up to 32 groups; a group takes kJoin neighbouring chunks, all loads in flight at once (one thread a channel and a
+// loop over 256 chunks took 70 us, this 5). A chunk with a reset inside passes nothing on, whatever comes in (not 0
+// times it: the state before a reset may be infinite or NaN).
+constexpr int kJoin = 16, kMaxChunks = 32 * kJoin;
 template <bool BACK>
 __global__ __launch_bounds__(1024) void scan_join(const Args a) {
-  __shared__ float sa[16][64], sb[16][64];
-  __shared__ unsigned char sc[16][64];
-  const ll nd = (ll)a.N * a.D, at = (ll)blockIdx.x * 64 + (threadIdx.x & 63);
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  __shared__ float sa[32][32], sb[32][32];
+  __shared__ unsigned char sc[32][32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const ll nd = (ll)a.N * a.D, at = (ll)blockIdx.x * 32 + lane;
   const bool on = at < nd;
   const int n = on ? (int)(at / a.D) : 0;
   const float* edge = BACK ? a.dlast : a.state;
@@ -155,6 +155,7 @@ __global__ __launch_bounds__(1024) void scan_join(const Args a) {
   sc[w][lane] = tc;
   __syncthreads();
   float s = first;
+#pragma unroll 8
   for (int k = 0; k < w; k++) s = sc[k][lane] ? sb[k][lane] : __builtin_fmaf(sa[k][lane], s, sb[k][lane]);
 #pragma unroll
   for (int k = 0; k < kJoin; k++) {
@@ -609,7 +610,7 @@ bool fits(const mjh_scan_desc& s, int v) {
 }
 
 constexpr int kWide = 2;
-constexpr ll kThreads = 262144, kFull = 65536, kLeast = 4;
+constexpr ll kThreads = 524288, kFull = 65536, kLeast = 2;
 
 int make_plan(const mjh_scan_desc* s, Plan& p) {
   if (!s) return refuse("scan: no description");
@@ -679,11 +680,11 @@ void launch_as(Kernel k, const Plan& p, hipStream_t s) {
       break;
     case kForwardAgg:
       scan_forward<T, GT, V, GV, BLEND, true, true><<<grid, block, 0, s>>>(a);
-      scan_join<false><<<dim3((unsigned)(((ll)a.N * a.D + 63) / 64)), dim3(64 * ((a.nchunk + kJoin - 1) / kJoin)), 0, s>>>(a);
+      scan_join<false><<<dim3((unsigned)(((ll)a.N * a.D + 31) / 32)), dim3(32 * ((a.nchunk + kJoin - 1) / kJoin)), 0, s>>>(a);
       break;
     case kBackwardAgg:
       scan_backward_agg<T, GT, V, GV, BLEND><<<grid, block, 0, s>>>(a);
-      scan_join<true><<<dim3((unsigned)(((ll)a.N * a.D + 63) / 64)), dim3(64 * ((a.nchunk + kJoin - 1) / kJoin)), 0, s>>>(a);
+      scan_join<true><<<dim3((unsigned)(((ll)a.N * a.D + 31) / 32)), dim3(32 * ((a.nchunk + kJoin - 1) / kJoin)), 0, s>>>(a);
       break;
     case kBackward:
       if (!p.heads) {
