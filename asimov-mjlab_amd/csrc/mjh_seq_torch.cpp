@@ -384,13 +384,25 @@ struct Norm {  // options of one call
 struct Rows {
   Tensor t;
   ll step = 0;
+  // rows one stride apart, neighbouring elements: a column range of a contiguous tensor, of any number of dimensions
+  bool even() const {
+    if (t.size(-1) > 1 && t.stride(-1) != 1) return false;
+    ll next = 0, rows = 1;  // what the stride of the next outer dimension has to be
+    for (int k = (int)t.dim() - 2; k >= 0; k--) {
+      if (t.size(k) == 1) continue;
+      if (rows > 1 && t.stride(k) != next) return false;
+      rows *= t.size(k);
+      next = t.stride(k) * t.size(k);
+    }
+    return true;
+  }
   explicit Rows(const Tensor& t0) : t(t0) {
     if (!t.defined()) return;
     const ll dim = t.size(-1);
     if (t.is_contiguous()) {
       step = dim;
-    } else if (t.dim() == 2 && (dim == 1 || t.stride(1) == 1)) {
-      step = t.size(0) > 1 ? t.stride(0) : 0;
+    } else if (even()) {
+      for (int k = (int)t.dim() - 2; k >= 0 && step == 0; k--) step = t.size(k) > 1 ? t.stride(k) : 0;
     } else {
       t = t.contiguous();
       step = dim;

@@ -499,10 +499,16 @@ def rng_args(env, site: str):
   """(seed, key, step-counter pointer) of the device random stream for one call
   site: draws differ per site, per env step (the counter is a device tensor the
   env step increments, so graph replays draw anew) and per host call."""
+  seed, key, ctr = rng_stream(env, site)
+  return ctypes.c_ulonglong(seed), ctypes.c_ulonglong(key), _ptr(ctr)
+
+
+def rng_stream(env, site: str) -> tuple[int, int, torch.Tensor]:
+  """``rng_args`` as (seed, key, step counter), as ``seqops.dropout`` takes them."""
   salt = env.__dict__.get("_rng_calls", 0) + 1
   env.__dict__["_rng_calls"] = salt
   key = (_site_hash(site) ^ (salt * 0x9E3779B97F4A7C15)) & 0xFFFFFFFFFFFFFFFF
-  return ctypes.c_ulonglong(env._rng_seed), ctypes.c_ulonglong(key), _ptr(env._rng_ctr)
+  return env._rng_seed, key, env._rng_ctr
 
 
 def uniform_draws(seed, key, ctr: torch.Tensor | None, n: int, device) -> torch.Tensor:

@@ -13,8 +13,10 @@ from __future__ import annotations
 import numpy as np
 import torch
 
+from mjlab_amd.envops import rng_stream
 from mjlab_amd.managers.manager_base import resolve_params
 from mjlab_amd.utils.buffers import CircularBuffer, DelayBuffer
+from mjlab_amd.utils.noise import DropoutNoiseCfg
 
 
 class ObservationManager:
@@ -161,7 +163,9 @@ class ObservationManager:
     obs_terms = {}
     for tname, tcfg in self._group_terms[group_name]:
       obs = tcfg.func(self._env, **tcfg.params).clone()  # noise/clip/scale act in place below
-      if tcfg.noise is not None:
+      if isinstance(tcfg.noise, DropoutNoiseCfg):
+        obs = tcfg.noise.apply(obs, rng_stream(self._env, f"observation_dropout/{group_name}/{tname}"))
+      elif tcfg.noise is not None:
         obs = tcfg.noise.apply(obs)
       if tcfg.clip:
         obs = obs.clip_(min=tcfg.clip[0], max=tcfg.clip[1])

@@ -1,3 +1,4 @@
+from mjlab_amd.rl.memory import PolicyMemory
 from mjlab_amd.rl.vecenv_wrapper import ObsDict, RslRlVecEnvWrapper
 
-__all__ = ["ObsDict", "RslRlVecEnvWrapper"]
+__all__ = ["ObsDict", "PolicyMemory", "RslRlVecEnvWrapper"]

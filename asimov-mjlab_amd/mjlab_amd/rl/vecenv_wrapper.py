@@ -7,6 +7,13 @@ Semantics otherwise follow the reference: reset at construction (rsl_rl never
 calls reset), optional action clipping, ``dones`` as long, and
 ``extras["time_outs"]`` for infinite-horizon tasks. With ``gather`` set, each
 step's outputs are also all-gathered across ranks (mjlab_amd.distributed).
+
+With ``memory`` (a PolicyMemory) set, the wrapper steps it on the ``memory_group``
+observations of every reset and env step, clears it at the envs that are done, and
+hands its features out as the observation ``"memory"`` next to the groups (not
+gathered: a learner on another rank forms them from the observations). The state
+before a rollout, which the learner's ``memory.forward`` needs, is
+``memory.state.clone()`` taken when the rollout begins.
 """
 
 from __future__ import annotations
@@ -14,6 +21,7 @@ from __future__ import annotations
 import torch
 
 from mjlab_amd.envs.manager_based_rl_env import Box, ManagerBasedRlEnv
+from mjlab_amd.rl.memory import PolicyMemory
 
 
 def _fresh_log(log: dict) -> dict:
@@ -41,7 +49,8 @@ class ObsDict(dict):
 
 
 class RslRlVecEnvWrapper:
-  def __init__(self, env: ManagerBasedRlEnv, clip_actions: float | None = None, gather: bool = False) -> None:
+  def __init__(self, env: ManagerBasedRlEnv, clip_actions: float | None = None, gather: bool = False,
+               memory: PolicyMemory | None = None, memory_group: str = "policy") -> None:
     self.env = env
     self.clip_actions = clip_actions
     self.num_envs = env.num_envs
@@ -54,7 +63,10 @@ class RslRlVecEnvWrapper:
 
       self._gather = StepGather()
     self._modify_action_space()
-    self.env.reset()
+    self.memory, self.memory_group = memory, memory_group
+    self._features: torch.Tensor | None = None
+    obs, _ = self.env.reset()
+    self._restart_memory(obs)
 
   @property
   def cfg(self):
@@ -91,12 +103,25 @@ class RslRlVecEnvWrapper:
   def seed(self, seed: int = -1) -> int:
     return self.env.seed(seed)
 
+  def _restart_memory(self, obs: dict) -> None:
+    """Every env's memory empty, then the first observation in it."""
+    if self.memory is not None:
+      self.memory.reset_state(self.num_envs)
+      self._features = self.memory.step(obs[self.memory_group])
+
+  def _with_memory(self, obs: dict) -> ObsDict:
+    if self._features is not None:
+      obs = {**obs, "memory": self._features}
+    return ObsDict(obs, [self.num_envs])
+
   def get_observations(self) -> ObsDict:
-    return ObsDict(self.env.observation_manager.compute(), [self.num_envs])
+    # the memory's features are those of the last reset or step: looking again does not advance it
+    return self._with_memory(self.env.observation_manager.compute())
 
   def reset(self):
     obs, extras = self.env.reset()
-    return ObsDict(obs, [self.num_envs]), extras
+    self._restart_memory(obs)
+    return self._with_memory(obs), extras
 
   def step(self, actions: torch.Tensor):
     if self.clip_actions is not None:
@@ -118,7 +143,9 @@ class RslRlVecEnvWrapper:
       extras["time_outs"] = truncated.clone()
     if self._gather is not None:
       extras["gathered"] = self._gather(obs, rew, terminated, truncated)
-    return ObsDict(obs, [self.num_envs]), rew, dones, extras
+    if self.memory is not None:  # a done env's obs is its next episode's first
+      self._features = self.memory.step(obs[self.memory_group], dones.bool())
+    return self._with_memory(obs), rew, dones, extras
 
   def close(self) -> None:
     return self.env.close()

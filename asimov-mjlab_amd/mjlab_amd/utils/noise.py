@@ -56,3 +56,24 @@ class GaussianNoiseCfg(NoiseCfg):
 
   def apply(self, data):
     return self._op(data, self._t(self.mean, data) + self._t(self.std, data) * torch.randn_like(data))
+
+
+@dataclass
+class DropoutNoiseCfg(NoiseCfg):
+  """Sensor dropout: each reading is lost (0) with probability ``p`` and passes unscaled
+  otherwise, whatever a lost reading holds (NaN included). Drawn from the env's device random
+  stream (``apply`` takes ``envops.rng_stream``'s triple), so a captured env step drops anew at every
+  replay; one launch (``seqops.dropout``). A group with such a term is assembled term by term."""
+
+  p: float = 0.0
+
+  def __post_init__(self):
+    if not 0.0 <= self.p <= 1.0:
+      raise ValueError(f"p ({self.p}) must be in [0, 1]")
+
+  def apply(self, data, stream=None):
+    from mjlab_amd import seqops
+
+    if stream is None:
+      raise ValueError("DropoutNoiseCfg needs the env's random stream (envops.rng_stream)")
+    return seqops.dropout(data, self.p, *stream, scale=1.0)
