@@ -245,11 +245,10 @@ __device__ __forceinline__ int wave_max(int v) {
   return __builtin_amdgcn_readfirstlane(v);
 }
 
-// AGG: the chunk's (product of a, result from state 0); else the outputs. AHEAD: loads of the next block under way
-// while this one is worked on, for chunked launches; with a thread for every channel of many rows the waves that
-// its registers cost are worth more.
-template <class T, class GT, int V, int GV, bool BLEND, bool AGG, bool AHEAD>
-__global__ __launch_bounds__(kBlock) void scan_forward(const Args a) {
+// What a chunk's steps do to the state that comes in, h -> A h + B: A = product of a, B = the result from 0. Bound by
+// the card's rate of reading (16,384 x 2,048 bfloat16: 24 us, 2.9 TB/s; 1 to 4 blocks of loads under way are the same).
+template <class T, class GT, int V, int GV, bool BLEND>
+__global__ __launch_bounds__(kBlock) void scan_forward_agg(const Args a) {
   const Where w = flat_where<V>(a);
   const Flags flags(w);
   const int c = blockIdx.y, t0 = c * a.chunk, t1 = min(a.T, t0 + a.chunk);
@@ -260,57 +259,94 @@ __global__ __launch_bounds__(kBlock) void scan_forward(const Args a) {
 #pragma unroll
   for (int v = 0; v < V; v++) s[v] = 0.f, prod[v] = 1.f;
   bool cut = false;
-  if (!AGG) incoming<V, false>(a, at, c, s);
+  for (int tb = t0; tb < stop; tb += kSteps) {
+    Block<T, GT, V, GV, true, false> b;
+    b.read(a, w, flags, tb < live, tb, t1);
+    const unsigned bits = flags.bits(a, w, b.flags);
+    if (__all(bits == 0 && tb + kSteps <= live)) {
+#pragma unroll
+      for (int j = 0; j < kSteps; j++)
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+          const Gate<BLEND> f((float)b.g[j].v[GV == 1 ? 0 : v]);
+          const float x = (float)b.x[j].v[v];
+          s[v] = __builtin_fmaf(f.a, s[v], BLEND ? f.b * x : x);
+          prod[v] *= f.a;
+        }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kSteps; j++) {
+        if (tb + j >= live) continue;
+        const bool reset = bits >> j & 1u;
+        cut |= reset;
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+          const Gate<BLEND> f((float)b.g[j].v[GV == 1 ? 0 : v]);
+          const float x = (float)b.x[j].v[v];
+          s[v] = __builtin_fmaf(f.a, reset ? 0.f : s[v], BLEND ? f.b * x : x);
+          prod[v] = reset ? 0.f : prod[v] * f.a;
+        }
+      }
+    }
+  }
+  if (!w.on) return;
+  store<float, V>(a.agg_a + c * nd + at, prod);
+  store<float, V>(a.agg_b + c * nd + at, s);
+  if (a.reset && w.d == 0) a.agg_cut[(ll)c * a.N + w.n] = cut;
+}
+
+// The outputs. AHEAD: loads of the next block under way while this one is worked on, for chunked launches; with a
+// thread for every channel of many rows the waves that its registers cost are worth more (24 x 4,096 x 256 bfloat16:
+// 33 us against 40).
+template <class T, class GT, int V, int GV, bool BLEND, bool AHEAD>
+__global__ __launch_bounds__(kBlock) void scan_forward(const Args a) {
+  const Where w = flat_where<V>(a);
+  const Flags flags(w);
+  const int c = blockIdx.y, t0 = c * a.chunk, t1 = min(a.T, t0 + a.chunk);
+  const int live = !w.on ? 0 : a.lengths ? min(a.lengths[w.n], t1) : t1;
+  const int stop = a.lengths ? wave_max(live) : t1;
+  const ll nd = (ll)a.N * a.D, at = (ll)w.n * a.D + w.d;
+  float s[V];
+  incoming<V, false>(a, at, c, s);
   T* ph = static_cast<T*>(a.h) + (ll)w.n * a.hn + w.d;
   Block<T, GT, V, GV, true, false> b, next;
   if (AHEAD && t0 < stop) b.read(a, w, flags, t0 < live, t0, t1);
   int tb = t0;
   for (; tb < stop; tb += kSteps) {
-    if (!AGG && a.kept && w.on) store<float, V>(a.kept + (ll)(tb / kSteps) * nd + at, s);
+    if (a.kept && w.on) store<float, V>(a.kept + (ll)(tb / kSteps) * nd + at, s);
     if (!AHEAD) b.read(a, w, flags, tb < live, tb, t1);
     if (AHEAD && tb + kSteps < stop) next.read(a, w, flags, tb + kSteps < live, tb + kSteps, t1);
     const unsigned bits = flags.bits(a, w, b.flags);
     if (__all(bits == 0 && tb + kSteps <= live)) {
 #pragma unroll
       for (int j = 0; j < kSteps; j++) {
-        float out[V];
 #pragma unroll
         for (int v = 0; v < V; v++) {
           const Gate<BLEND> f((float)b.g[j].v[GV == 1 ? 0 : v]);
           const float x = (float)b.x[j].v[v];
-          out[v] = s[v] = __builtin_fmaf(f.a, s[v], BLEND ? f.b * x : x);
-          if (AGG) prod[v] *= f.a;
+          s[v] = __builtin_fmaf(f.a, s[v], BLEND ? f.b * x : x);
         }
-        if (!AGG) store<T, V>(ph + (ll)(tb + j) * a.ht, out);
+        store<T, V>(ph + (ll)(tb + j) * a.ht, s);
       }
     } else {  // a reset, a row's end or the last step inside
 #pragma unroll
       for (int j = 0; j < kSteps; j++) {
-        const bool in = tb + j < live, reset = bits >> j & 1u;
         float out[V];
 #pragma unroll
         for (int v = 0; v < V; v++) {
           out[v] = 0.f;
-          if (in) {
+          if (tb + j < live) {
             const Gate<BLEND> f((float)b.g[j].v[GV == 1 ? 0 : v]);
             const float x = (float)b.x[j].v[v];
-            out[v] = s[v] = __builtin_fmaf(f.a, reset ? 0.f : s[v], BLEND ? f.b * x : x);
-            if (AGG) prod[v] = reset ? 0.f : prod[v] * f.a;
+            out[v] = s[v] = __builtin_fmaf(f.a, bits >> j & 1u ? 0.f : s[v], BLEND ? f.b * x : x);
           }
         }
-        if (AGG) cut |= in && reset;
-        if (!AGG && w.on && tb + j < t1) store<T, V>(ph + (ll)(tb + j) * a.ht, out);
+        if (w.on && tb + j < t1) store<T, V>(ph + (ll)(tb + j) * a.ht, out);
       }
     }
     if (AHEAD) b = next;
   }
   if (!w.on) return;
-  if (AGG) {
-    store<float, V>(a.agg_a + c * nd + at, prod);
-    store<float, V>(a.agg_b + c * nd + at, s);
-    if (a.reset && w.d == 0) a.agg_cut[(ll)c * a.N + w.n] = cut;
-    return;
-  }
   for (; tb < t1; tb += kSteps) {  // beyond the rows' lengths: nothing to read
     if (a.kept) store<float, V>(a.kept + (ll)(tb / kSteps) * nd + at, s);
     const float none[V] = {};
@@ -334,37 +370,32 @@ __global__ __launch_bounds__(kBlock) void scan_backward_agg(const Args a) {
 #pragma unroll
   for (int v = 0; v < V; v++) e[v] = 0.f, prod[v] = 1.f;
   bool cut = false;
-  if (stop > t0) {
-    Block<T, GT, V, GV, false, true> b, next;
-    int tb = t0 + (stop - 1 - t0) / kSteps * kSteps;
+  for (int tb = t0 + (max(stop - t0, 0) + kSteps - 1) / kSteps * kSteps - kSteps; tb >= t0; tb -= kSteps) {
+    Block<T, GT, V, GV, false, true> b;
     b.read(a, w, flags, tb < live, tb, t1);
-    for (; tb >= t0; tb -= kSteps) {
-      if (tb > t0) next.read(a, w, flags, tb - kSteps < live, tb - kSteps, t1);
-      const unsigned bits = flags.bits(a, w, b.flags);
-      if (__all(bits == 0 && tb + kSteps <= live)) {
+    const unsigned bits = flags.bits(a, w, b.flags);
+    if (__all(bits == 0 && tb + kSteps <= live)) {
 #pragma unroll
-        for (int j = kSteps - 1; j >= 0; j--)
+      for (int j = kSteps - 1; j >= 0; j--)
 #pragma unroll
-          for (int v = 0; v < V; v++) {
-            const Gate<BLEND> f((float)b.g[j].v[GV == 1 ? 0 : v]);
-            e[v] = f.a * ((float)b.dh[j].v[v] + e[v]);
-            prod[v] *= f.a;
-          }
-      } else {
+        for (int v = 0; v < V; v++) {
+          const Gate<BLEND> f((float)b.g[j].v[GV == 1 ? 0 : v]);
+          e[v] = f.a * ((float)b.dh[j].v[v] + e[v]);
+          prod[v] *= f.a;
+        }
+    } else {
 #pragma unroll
-        for (int j = kSteps - 1; j >= 0; j--) {
-          if (tb + j >= live) continue;
-          const bool reset = bits >> j & 1u;
+      for (int j = kSteps - 1; j >= 0; j--) {
+        if (tb + j >= live) continue;
+        const bool reset = bits >> j & 1u;
+        cut |= reset;
 #pragma unroll
-          for (int v = 0; v < V; v++) {
-            const Gate<BLEND> f((float)b.g[j].v[GV == 1 ? 0 : v]);
-            e[v] = reset ? 0.f : f.a * ((float)b.dh[j].v[v] + e[v]);
-            prod[v] = reset ? 0.f : prod[v] * f.a;
-          }
-          cut |= reset;
+        for (int v = 0; v < V; v++) {
+          const Gate<BLEND> f((float)b.g[j].v[GV == 1 ? 0 : v]);
+          e[v] = reset ? 0.f : f.a * ((float)b.dh[j].v[v] + e[v]);
+          prod[v] = reset ? 0.f : prod[v] * f.a;
         }
       }
-      b = next;
     }
   }
   if (!w.on) return;
@@ -674,12 +705,12 @@ void launch_as(Kernel k, const Plan& p, hipStream_t s) {
   switch (k) {
     case kForward:
       if (a.nchunk > 1)
-        scan_forward<T, GT, V, GV, BLEND, false, true><<<grid, block, 0, s>>>(a);
+        scan_forward<T, GT, V, GV, BLEND, true><<<grid, block, 0, s>>>(a);
       else
-        scan_forward<T, GT, V, GV, BLEND, false, false><<<grid, block, 0, s>>>(a);
+        scan_forward<T, GT, V, GV, BLEND, false><<<grid, block, 0, s>>>(a);
       break;
     case kForwardAgg:
-      scan_forward<T, GT, V, GV, BLEND, true, true><<<grid, block, 0, s>>>(a);
+      scan_forward_agg<T, GT, V, GV, BLEND><<<grid, block, 0, s>>>(a);
       scan_join<false><<<dim3((unsigned)(((ll)a.N * a.D + 31) / 32)), dim3(32 * ((a.nchunk + kJoin - 1) / kJoin)), 0, s>>>(a);
       break;
     case kBackwardAgg:
