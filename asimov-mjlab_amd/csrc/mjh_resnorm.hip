@@ -48,6 +48,7 @@ struct Args {
   Drop drop;
   float eps, inv;  // inv = 1 / D
   int R, D, layer, act, post, pre;
+  ll row0;    // long rows: the first row of this launch
   int tpr;    // lanes that hold a row
   int parts;  // workgroups (long rows: strands of rows) of the backward pass
 };
@@ -546,8 +547,8 @@ __global__ __launch_bounds__(256) void resnorm_stream(const Args a) {
   constexpr int N = 16 / (int)sizeof(T);
   __shared__ float shared[2][4];
   extern __shared__ float kept[];  // slot by slot: (N, slots)
-  if (a.ctr_out && blockIdx.x == 0 && threadIdx.x == 0) *a.ctr_out = a.drop.ctr ? *a.drop.ctr : 0;
-  const ll row = blockIdx.x;
+  if (a.ctr_out && a.row0 + blockIdx.x == 0 && threadIdx.x == 0) *a.ctr_out = a.drop.ctr ? *a.drop.ctr : 0;
+  const ll row = a.row0 + blockIdx.x;
   const bool block = a.y != nullptr;
   const unsigned long long base = a.drop.thr ? drop_base(a.drop) : 0;
   const int slots = a.D / N + a.D % N;
@@ -704,7 +705,7 @@ template <class T, bool BLOCK, bool BIAS>
 __global__ __launch_bounds__(256) void resnorm_rows(const Args a) {
   constexpr int N = kBack;
   __shared__ float shared[4][8];
-  const ll row = blockIdx.x;
+  const ll row = a.row0 + blockIdx.x;
   const unsigned long long base = BLOCK && a.drop.thr ? drop_base(a.drop) : 0;
   const auto st = load<float, 4>(a.stats + row * 4);
   const int slots = a.D / N + a.D % N;
@@ -1020,10 +1021,16 @@ void launch_backward_rows(const Args& a, hipStream_t s) {
   if (sizeof(T) == 4 || a.tpr <= 256) return launch_backward<T, FULL, 256, BLOCK, BIAS>(a, s);
   if constexpr (sizeof(T) == 2) launch_backward<T, FULL, 512, BLOCK, BIAS>(a, s);
 }
+// One workgroup a row, in launches whose threads stay below 2^32 (a loop over rows in the kernels cost a tenth).
+template <class F>
+void by_row(Args a, F launch_rows) {
+  constexpr ll most = 1 << 23;
+  for (; a.row0 < a.R; a.row0 += most) launch_rows(a, (unsigned)std::min<ll>(most, a.R - a.row0));
+}
 template <class T, bool BLOCK, bool BIAS>
 void launch_backward_as(const Args& a, bool streams, hipStream_t s) {
   if (streams) {
-    resnorm_rows<T, BLOCK, BIAS><<<dim3(a.R), dim3(256), 0, s>>>(a);
+    by_row(a, [&](const Args& b, unsigned rows) { resnorm_rows<T, BLOCK, BIAS><<<dim3(rows), dim3(256), 0, s>>>(b); });
     resnorm_columns<T, BLOCK, BIAS><<<dim3((a.D / kBack + a.D % kBack + 63) / 64, a.parts), dim3(64), 0, s>>>(a);
   } else if (a.tpr * kPer == a.D) {
     launch_backward_rows<T, true, BLOCK, BIAS>(a, s);
@@ -1039,9 +1046,11 @@ void launch_type(const mjh_resnorm_desc& d, const Args& a, bool back, hipStream_
   else if (back)
     bias ? launch_backward_as<T, false, true>(a, streams, s) : launch_backward_as<T, false, false>(a, streams, s);
   else if (streams && a.D <= 8192)
-    resnorm_stream<T, true><<<dim3(a.R), dim3(256), 4 * (16 / sizeof(T)) * (a.D / (16 / sizeof(T)) + a.D % (16 / sizeof(T))), s>>>(a);
+    by_row(a, [&](const Args& b, unsigned rows) {
+      resnorm_stream<T, true><<<dim3(rows), dim3(256), 4 * (16 / sizeof(T)) * (a.D / (16 / sizeof(T)) + a.D % (16 / sizeof(T))), s>>>(b);
+    });
   else if (streams)
-    resnorm_stream<T, false><<<dim3(a.R), dim3(256), 0, s>>>(a);
+    by_row(a, [&](const Args& b, unsigned rows) { resnorm_stream<T, false><<<dim3(rows), dim3(256), 0, s>>>(b); });
   else
     a.tpr * kPer == a.D ? launch_forward_rows<T, true>(a, s) : launch_forward_rows<T, false>(a, s);
 }

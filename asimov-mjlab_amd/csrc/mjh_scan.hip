@@ -647,7 +647,7 @@ int make_plan(const mjh_scan_desc* s, Plan& p) {
   if (!s) return refuse("scan: no description");
   if (s->T < 1 || s->N < 1 || s->D < 1 || s->G < 1) return refuse("scan: T, N, D and G must be positive");
   if (s->D % s->G) return refuse("scan: G must divide D");
-  if ((ll)s->N * s->D > 0x7fffffffll) return refuse("scan: N * D must be below 2^31");
+  if ((ll)s->N * s->D > 0x7fffffffll || s->T > 1 << 30) return refuse("scan: N * D must be below 2^31, T at most 2^30");
   if (s->dtype < 0 || s->dtype > 2 || (s->gtype != s->dtype && s->gtype != MJH_F32))
     return refuse("scan: the gate must have x's type or float32");
   if (s->mode != MJH_SCAN_DECAY && s->mode != MJH_SCAN_BLEND) return refuse("scan: unknown mode");

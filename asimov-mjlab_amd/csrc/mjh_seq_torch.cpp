@@ -137,7 +137,7 @@ void check_scan(const char* name, const Tensor& x, const Tensor& gate, const Ten
   same_device(name, x, "reset", reset);
   same_device(name, x, "lengths", lengths);
   known_device(name, x);
-  if (n * d > 0x7fffffff || (dims == 3 && x.size(0) > 0x7fffffff)) refuse(name, ": N * D and T must be below 2^31");
+  if (n * d > 0x7fffffff || (dims == 3 && x.size(0) > 1 << 30)) refuse(name, ": N * D must be below 2^31 and T at most 2^30");
 }
 
 mjh_scan_desc scan_desc(const Tensor& x, const Tensor& gate, const Tensor& reset, const Tensor& lengths, int mode) {
@@ -242,6 +242,19 @@ py::object gated_scan(const Tensor& x, const Tensor& gate, const Maybe& state_, 
   return py::make_tuple(std::move(o.h), std::move(o.last));
 }
 
+// whether two tensors' memory ranges meet
+bool overlap(const Tensor& s, const Tensor& t) {
+  if (!s.numel() || !t.numel()) return false;
+  auto range = [](const Tensor& u) {
+    ll last = 0;
+    for (int k = 0; k < (int)u.dim(); k++) last += (u.size(k) - 1) * u.stride(k);
+    const char* p = static_cast<const char*>(u.data_ptr());
+    return std::make_pair(p, p + (last + 1) * (ll)u.element_size());
+  };
+  const auto a = range(s), b = range(t);
+  return a.first < b.second && b.first < a.second;
+}
+
 py::object gated_step(const Tensor& x0, const Tensor& gate0, const Maybe& state_, const Maybe& reset_,
                       int mode, const Maybe& out_) {
   static const char* name = "gated_step";
@@ -255,15 +268,10 @@ py::object gated_step(const Tensor& x0, const Tensor& gate0, const Maybe& state_
     if (out.sizes() != state.sizes() || out.scalar_type() != at::kFloat || !out.is_contiguous() || out.device() != state.device())
       refuse(name, ": out must be contiguous float32 of shape ", state.sizes(), " on ", state.device());
     TORCH_CHECK(!wants_grad({&out}), "gated_step: out requires a gradient");
-    // rows that another thread may still read must not be written
-    const auto apart = std::llabs((ll)((char*)out.data_ptr() - (char*)state.data_ptr()));
-    const bool same = apart == 0 && state.is_contiguous();
-    if (!same && out.numel() && out.storage().is_alias_of(state.storage())) {
-      ll span = 1;
-      for (int k = 0; k < 2; k++) span += (state.size(k) - 1) * state.stride(k);
-      const char *a = (char*)out.data_ptr(), *b = (char*)state.data_ptr();
-      if (a < b + 4 * span && b < a + 4 * out.numel()) refuse(name, ": out and state overlap without being the same rows");
-    }
+    // what another thread may still read must not be written
+    if (!(out.data_ptr() == state.data_ptr() && state.is_contiguous()) && overlap(out, state))
+      refuse(name, ": out and state overlap without being the same rows");
+    if (overlap(out, x0) || overlap(out, gate0) || (reset.defined() && overlap(out, reset))) refuse(name, ": out overlaps an input");
   }
   if (!x0.is_cuda() || x0.numel() == 0) return py::none();
   c10::DeviceGuard guard(x0.device());

@@ -149,6 +149,9 @@ def test_step_refusals_and_formula():
   buf = torch.zeros(4, 4)
   with pytest.raises(ValueError, match="overlap"):
     seqops.gated_step(x, g, buf[:3], out=buf[1:])
+  both = torch.zeros(3, 8)
+  with pytest.raises(ValueError, match="overlaps an input"):
+    seqops.gated_step(both[:, :4], g, s, out=both.view(6, 4)[:3])
   reset = torch.tensor([True, False, False])
   h, last = seqops.gated_step(x, g, s, reset)
   ref = seq_ref.scan(x[None], g[None], s, reset[None])
