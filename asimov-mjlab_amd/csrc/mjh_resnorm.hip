@@ -367,22 +367,40 @@ __global__ __launch_bounds__(threads_of(TPR)) void resnorm_backward(const Args a
   for (int q = 0; q < kSums; q++)
 #pragma unroll
     for (int k = 0; k < kPer; k++) sum[q][k] = 0.f;
-  // No row is loaded ahead (98,304 x 256 bfloat16: 85 us against 108 with it).
+  // The row ahead is loaded only where one workgroup fills a CU, which then waits for its loads and barriers alone
+  // (8,192 x 4,096 bfloat16: 165 us, 194 without; 98,304 x 256: 108 us with it, 85 without).
+  constexpr bool AHEAD = TPR > 256;
+  auto fetch = [&](ll row, Pack<float, 4>& st, T (&r)[kPer], T (&y)[kPer], T (&g)[kPer], T (&ds)[kPer], T (&dn)[kPer]) {
+    const bool on = row < a.R;
+    if (on) st = load<float, 4>(a.stats + row * 4);
+    if (BLOCK) {
+      at.read(a.y, row, a.ys, on, y);
+      if (a.gate) at.read(a.gate, row, a.gs, on, g);
+    }
+    if (a.dn) {
+      at.read(a.r, row, a.rs, on, r);
+      at.read(a.dn, row, a.dns, on, dn);
+    }
+    if (a.ds) at.read(a.ds, row, a.dss, on, ds);
+  };
+  T next_r[kPer], next_y[kPer], next_g[kPer], next_ds[kPer], next_dn[kPer];
+  Pack<float, 4> next_st{};
+  if constexpr (AHEAD) fetch((ll)blockIdx.x * R::kGroups + at.group, next_st, next_r, next_y, next_g, next_ds, next_dn);
   for (ll first = (ll)blockIdx.x * R::kGroups; first < a.R; first += (ll)gridDim.x * R::kGroups) {
     const ll row = first + at.group;
     const bool on = row < a.R;
     T raw_r[kPer], raw_y[kPer], raw_g[kPer], raw_ds[kPer], raw_dn[kPer];
     Pack<float, 4> st{};
-    if (on) st = load<float, 4>(a.stats + row * 4);
-    if (BLOCK) {
-      at.read(a.y, row, a.ys, on, raw_y);
-      if (a.gate) at.read(a.gate, row, a.gs, on, raw_g);
+    if constexpr (AHEAD) {
+      st = next_st;
+#pragma unroll
+      for (int k = 0; k < kPer; k++) {
+        raw_r[k] = next_r[k]; raw_y[k] = next_y[k]; raw_g[k] = next_g[k]; raw_ds[k] = next_ds[k]; raw_dn[k] = next_dn[k];
+      }
+      fetch(row + (ll)gridDim.x * R::kGroups, next_st, next_r, next_y, next_g, next_ds, next_dn);
+    } else {
+      fetch(row, st, raw_r, raw_y, raw_g, raw_ds, raw_dn);
     }
-    if (a.dn) {
-      at.read(a.r, row, a.rs, on, raw_r);
-      at.read(a.dn, row, a.dns, on, raw_dn);
-    }
-    if (a.ds) at.read(a.ds, row, a.dss, on, raw_ds);
     const float mean = st.v[0], rstd = st.v[1], pre_mean = st.v[2], pre_rstd = st.v[3];
     bool in[kPer];
 #pragma unroll
@@ -999,9 +1017,19 @@ void launch_forward(const Args& a, hipStream_t s) {
   const ll need = (a.R + groups - 1) / groups;
   resnorm_forward<T, FULL, TPR><<<dim3((unsigned)std::min<ll>(need, 256 * 32 / waves)), dim3(TPR > 64 ? a.tpr : 256), 0, s>>>(a);
 }
+// As many parts as are resident, where the rows are enough: a part takes the same share of the rows, so one more round
+// of a few workgroups costs a whole round (98,304 x 99 floats, 2 waves a SIMD by their registers: 93 us as 2 workgroups
+// a CU, 119 as 3; 98,304 x 256 bfloat16, 3 waves a SIMD: 99 and 86). At most parts_of(), which the workspace holds.
 template <class T, bool FULL, int TPR, bool BLOCK, bool BIAS>
-void launch_backward(const Args& a, hipStream_t s) {
-  resnorm_backward<T, FULL, TPR, BLOCK, BIAS><<<dim3(a.parts), dim3(TPR > 64 ? a.tpr : 256), 0, s>>>(a);
+void launch_backward(Args& a, hipStream_t s) {
+  static const int waves_simd = [] {
+    int n = 0;
+    const bool ok = hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, resnorm_backward<T, FULL, TPR, BLOCK, BIAS>, 256, 0) == hipSuccess;
+    return ok && n ? n : 2;
+  }();
+  const int threads = TPR > 64 ? a.tpr : 256;
+  a.parts = std::min(a.parts, 256 * std::max(1, waves_simd * 256 / threads));
+  resnorm_backward<T, FULL, TPR, BLOCK, BIAS><<<dim3(a.parts), dim3(threads), 0, s>>>(a);
 }
 template <class T, bool FULL>
 void launch_forward_rows(const Args& a, hipStream_t s) {
@@ -1013,7 +1041,7 @@ void launch_forward_rows(const Args& a, hipStream_t s) {
   if constexpr (sizeof(T) == 2) launch_forward<T, FULL, 512>(a, s);
 }
 template <class T, bool FULL, bool BLOCK, bool BIAS>
-void launch_backward_rows(const Args& a, hipStream_t s) {
+void launch_backward_rows(Args& a, hipStream_t s) {
   if (a.tpr == 8) return launch_backward<T, FULL, 8, BLOCK, BIAS>(a, s);
   if (a.tpr == 16) return launch_backward<T, FULL, 16, BLOCK, BIAS>(a, s);
   if (a.tpr == 32) return launch_backward<T, FULL, 32, BLOCK, BIAS>(a, s);
@@ -1028,7 +1056,7 @@ void by_row(Args a, F launch_rows) {
   for (; a.row0 < a.R; a.row0 += most) launch_rows(a, (unsigned)std::min<ll>(most, a.R - a.row0));
 }
 template <class T, bool BLOCK, bool BIAS>
-void launch_backward_as(const Args& a, bool streams, hipStream_t s) {
+void launch_backward_as(Args& a, bool streams, hipStream_t s) {
   if (streams) {
     by_row(a, [&](const Args& b, unsigned rows) { resnorm_rows<T, BLOCK, BIAS><<<dim3(rows), dim3(256), 0, s>>>(b); });
     resnorm_columns<T, BLOCK, BIAS><<<dim3((a.D / kBack + a.D % kBack + 63) / 64, a.parts), dim3(64), 0, s>>>(a);
@@ -1039,7 +1067,7 @@ void launch_backward_as(const Args& a, bool streams, hipStream_t s) {
   }
 }
 template <class T>
-void launch_type(const mjh_resnorm_desc& d, const Args& a, bool back, hipStream_t s) {
+void launch_type(const mjh_resnorm_desc& d, Args& a, bool back, hipStream_t s) {
   const bool streams = long_row(d.D, d.dtype), bias = wants_bias(d);
   if (back && a.y)
     bias ? launch_backward_as<T, true, true>(a, streams, s) : launch_backward_as<T, true, false>(a, streams, s);
@@ -1054,7 +1082,7 @@ void launch_type(const mjh_resnorm_desc& d, const Args& a, bool back, hipStream_
   else
     a.tpr * kPer == a.D ? launch_forward_rows<T, true>(a, s) : launch_forward_rows<T, false>(a, s);
 }
-void launch(const mjh_resnorm_desc& d, const Args& a, bool back, hipStream_t s) {
+void launch(const mjh_resnorm_desc& d, Args& a, bool back, hipStream_t s) {
   if (d.dtype == MJH_F32)
     launch_type<float>(d, a, back, s);
   else if (d.dtype == MJH_BF16)
@@ -1092,7 +1120,8 @@ long long mjh_resnorm_workspace(const mjh_resnorm_desc* d) {
 int mjh_resnorm_forward(const mjh_resnorm_desc* d, void* stream) {
   if (int rc = check(d)) return rc;
   if ((d->y && !d->s) || (d->pre && !d->n) || (!d->y && !d->pre)) return refuse("residual norm forward: an output is missing");
-  launch(*d, args_of(*d), false, reinterpret_cast<hipStream_t>(stream));
+  Args a = args_of(*d);
+  launch(*d, a, false, reinterpret_cast<hipStream_t>(stream));
   return launched();
 }
 
