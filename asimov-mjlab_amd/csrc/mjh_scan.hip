@@ -117,10 +117,14 @@ struct Gate {
 
 // The chunks' results become the state that comes into each chunk (forward: from the chunks before it; BACK: the
 // gradient from the chunks after it), written over the chunk's own result in agg_b. A workgroup holds 32 channels
-// by up to 32 groups; a group takes kJoin neighbouring chunks, all loads in flight at once (one thread a channel and a
-// loop over 256 chunks took 70 us, this 5). A chunk with a reset inside passes nothing on, whatever comes in (not 0
-// times it: the state before a reset may be infinite or NaN).
+// by up to 32 groups; a group takes kJoin neighbouring chunks, all loads in flight at once (2,048 channels by 512
+// chunks: 8.3 us; 16 channels by 64 groups 9.3, 8 by 64 14; one thread a channel and a loop over 256 chunks 70). A
+// chunk with a reset inside passes nothing on, whatever comes in (not 0 times it: the state before a reset may be
+// infinite or NaN), and a state of 0 adds nothing, however far the product of the gates overflows.
 constexpr int kJoin = 16, kMaxChunks = 32 * kJoin;
+__device__ __forceinline__ float carry(float p, float s, float q, bool cut) {
+  return cut || s == 0.f ? q : __builtin_fmaf(p, s, q);
+}
 template <bool BACK>
 __global__ __launch_bounds__(1024) void scan_join(const Args a) {
   __shared__ float sa[32][32], sb[32][32];
@@ -146,7 +150,7 @@ __global__ __launch_bounds__(1024) void scan_join(const Args a) {
   bool tc = false;
 #pragma unroll
   for (int k = 0; k < kJoin; k++) {
-    tb = cut[k] ? q[k] : __builtin_fmaf(p[k], tb, q[k]);
+    tb = carry(p[k], tb, q[k], cut[k]);
     ta *= p[k];
     tc |= cut[k];
   }
@@ -156,13 +160,13 @@ __global__ __launch_bounds__(1024) void scan_join(const Args a) {
   __syncthreads();
   float s = first;
 #pragma unroll 8
-  for (int k = 0; k < w; k++) s = sc[k][lane] ? sb[k][lane] : __builtin_fmaf(sa[k][lane], s, sb[k][lane]);
+  for (int k = 0; k < w; k++) s = carry(sa[k][lane], s, sb[k][lane], sc[k][lane]);
 #pragma unroll
   for (int k = 0; k < kJoin; k++) {
     const int i = w * kJoin + k;
     if (!on || i >= a.nchunk) break;
     a.agg_b[(BACK ? a.nchunk - 1 - i : i) * nd + at] = s;
-    s = cut[k] ? q[k] : __builtin_fmaf(p[k], s, q[k]);
+    s = carry(p[k], s, q[k], cut[k]);
   }
 }
 
@@ -220,16 +224,24 @@ struct Block {
     const T* px = static_cast<const T*>(a.x) + (ll)w.n * a.xn + w.d;
     const GT* pg = static_cast<const GT*>(a.gate) + (ll)w.n * a.gn + w.g;
     const T* pd = static_cast<const T*>(a.dh) + (ll)w.n * a.dhn + w.d;
+    px += tb * a.xt;
+    pg += tb * a.gt;
 #pragma unroll
     for (int j = 0; j < kSteps; j++) {
-      const ll t = min(tb + j, end - 1);
-      if constexpr (X) x[j] = load<T, V>(px + t * a.xt);
-      g[j] = load<GT, GV>(pg + t * a.gt);
+      if constexpr (X) x[j] = load<T, V>(px);
+      g[j] = load<GT, GV>(pg);
+      if (j + 1 == kSteps) break;
+      if constexpr (X) px += tb + j + 1 < end ? a.xt : 0;
+      pg += tb + j + 1 < end ? a.gt : 0;
     }
     if constexpr (DH) {
       if (a.dh) {
+        pd += tb * a.dht;
 #pragma unroll
-        for (int j = 0; j < kSteps; j++) dh[j] = load<T, V>(pd + (ll)min(tb + j, end - 1) * a.dht);
+        for (int j = 0; j < kSteps; j++) {
+          dh[j] = load<T, V>(pd);
+          if (j + 1 < kSteps) pd += tb + j + 1 < end ? a.dht : 0;
+        }
       } else {
 #pragma unroll
         for (int j = 0; j < kSteps; j++) dh[j] = Pack<T, V>{};
@@ -248,7 +260,7 @@ __device__ __forceinline__ int wave_max(int v) {
 // What a chunk's steps do to the state that comes in, h -> A h + B: A = product of a, B = the result from 0. Bound by
 // the card's rate of reading (16,384 x 2,048 bfloat16: 24 us, 2.9 TB/s; 1 to 4 blocks of loads under way are the same).
 template <class T, class GT, int V, int GV, bool BLEND>
-__global__ __launch_bounds__(kBlock) void scan_forward_agg(const Args a) {
+__global__ __launch_bounds__(kBlock, 8) void scan_forward_agg(const Args a) {
   const Where w = flat_where<V>(a);
   const Flags flags(w);
   const int c = blockIdx.y, t0 = c * a.chunk, t1 = min(a.T, t0 + a.chunk);
@@ -359,7 +371,7 @@ __global__ __launch_bounds__(kBlock) void scan_forward(const Args a) {
 
 // The chunk's effect on the gradient that comes in from the steps after it.
 template <class T, class GT, int V, int GV, bool BLEND>
-__global__ __launch_bounds__(kBlock) void scan_backward_agg(const Args a) {
+__global__ __launch_bounds__(kBlock, 8) void scan_backward_agg(const Args a) {
   const Where w = flat_where<V>(a);
   const Flags flags(w);
   const int c = blockIdx.y, t0 = c * a.chunk, t1 = min(a.T, t0 + a.chunk);
