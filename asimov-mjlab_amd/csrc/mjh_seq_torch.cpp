@@ -293,6 +293,7 @@ py::object gated_step(const Tensor& x0, const Tensor& gate0, const Maybe& state_
   s.T = 1; s.N = (int)x.size(0); s.D = (int)x.size(1); s.G = (int)gate.size(1);
   s.dtype = type_of(x); s.gtype = type_of(gate); s.mode = mode;
   check(lib.scan_step(&s, stream_of(x)), "mjh_scan_step");
+  if (out_.has_value() && !out.is_inference()) out.unsafeGetTensorImpl()->bump_version();  // written in place
   return py::make_tuple(std::move(h), std::move(out));
 }
 
@@ -313,7 +314,7 @@ Tensor dropout_run(const Tensor& x0, double scale, const Stream& r, const Tensor
   Tensor x = x0;
   ll rows = 1, cols = x.numel(), xs = 0;
   if (!x.is_contiguous()) {
-    if (x.dim() == 2 && x.stride(1) == 1 && x.stride(0) > 0) {
+    if (x.dim() == 2 && x.stride(1) == 1 && x.stride(0) > 0 && x.size(1) <= 0x7fffffff) {
       rows = x.size(0); cols = x.size(1); xs = x.stride(0);
     } else {
       x = x.contiguous();

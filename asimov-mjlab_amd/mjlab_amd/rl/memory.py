@@ -81,12 +81,14 @@ class PolicyMemory(nn.Module):
     return n, torch.stack(last)
 
   def reset_state(self, num_envs: int) -> None:
-    """Zero state for ``num_envs`` envs, at the same address as before if their number has not changed."""
-    if self.state is not None and self.state.shape[1] == num_envs:
+    """Zero state for ``num_envs`` envs, at the same address as before if neither their number nor the module's
+    device has changed."""
+    device = self.embed.weight.device
+    if self.state is not None and self.state.shape[1] == num_envs and self.state.device == device:
       self.state.zero_()
     else:
-      p = self.embed.weight
-      self.state = torch.zeros((self.num_layers, num_envs, self.dim), dtype=torch.float32, device=p.device)
+      with torch.inference_mode(False):  # a rollout's inference mode does not bind later ones to it
+        self.state = torch.zeros((self.num_layers, num_envs, self.dim), dtype=torch.float32, device=device)
 
   @torch.no_grad()
   def step(self, obs: torch.Tensor, reset: torch.Tensor | None = None) -> torch.Tensor:

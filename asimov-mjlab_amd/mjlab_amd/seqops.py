@@ -52,7 +52,7 @@ def _scan_torch(x, gate, state, reset, lengths, mode: str):
   """The recurrence in torch operations, step by step (differentiable)."""
   t, n, d = x.shape
   wide = torch.promote_types(x.dtype, torch.float32)
-  h = torch.zeros((n, d), dtype=wide, device=x.device) if state is None else state.to(wide)
+  h = torch.zeros((n, d), dtype=wide, device=x.device) if state is None else state.to(wide, copy=True)
   k = d // gate.shape[2] if d else 1
   out = []
   for i in range(t):
@@ -76,7 +76,9 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor | None =
   Channel ``d`` of row ``n`` uses gate ``d // (D // G)`` (one gate per channel, or one per head):
 
   * ``mode="blend"``: ``h_t = sigmoid(gate) h' + sigmoid(-gate) x_t``
-  * ``mode="decay"``: ``h_t = gate h' + x_t`` (any real gate)
+  * ``mode="decay"``: ``h_t = gate h' + x_t`` (any real gate; a long scan of few channels is cut into
+    chunks, over whose steps the product of the gates has to stay in float32's range, as that of gates
+    in [-1, 1] does, wherever a state comes in)
 
   with ``h' = 0`` where ``reset[t, n]`` (step t is the first of an episode: the ``dones`` of the env
   step that returned its observation), else the row's previous state; ``state`` (None: 0) precedes
@@ -87,7 +89,9 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor | None =
   decays: its steps below 1 are 2^-8).
 
   The gradients of x, gate and state start from the float32 states, not from the rounded h. The
-  backward pass needs ``ceil(T / 8) N D`` kept float32 values. Time: one pass over the tensors."""
+  backward pass needs ``ceil(T / 8) N D`` kept float32 values. Time: one pass over the tensors; with
+  fewer than 65,536 channels (times 2 where neighbours are read in pairs) in N D, x, gate and the
+  gradient of h are read a second time, by the launch that forms the chunks' effects."""
   out = (_EXT or _ext()).gated_scan(x, gate, state, reset, lengths, _MODES.get(mode, -1))
   return _scan_torch(x, gate, state, reset, lengths, mode) if out is None else out
 

@@ -115,6 +115,23 @@ def test_reset_leaves_no_trace(t, mode):
   assert torch.equal(back[4], clean[4])
 
 
+def test_growing_gates_of_an_empty_state():
+  """Gates whose product over a chunk overflows add nothing to a state (gradient) of 0."""
+  x = torch.zeros(4001, 1, 6, device="cuda")
+  gate = torch.full((4001, 1, 6), 2.0, device="cuda")
+  x[3990:, 0, 1] = 1.0
+  dh = torch.zeros_like(x)
+  dh[:10, 0, 2] = 1.0
+  h, last, dx, dgate, dstate = run_scan(x, gate, torch.zeros(1, 6, device="cuda"), None, None, dh, torch.zeros(1, 6, device="cuda"), "decay")
+  want = torch.zeros(4001, 6, device="cuda")
+  want[3990:, 1] = 2.0 ** torch.arange(1, 12, device="cuda") - 1.0  # sums of powers of two: exact
+  assert torch.equal(h[:, 0], want) and torch.equal(last[0], want[-1])
+  back = torch.zeros(4001, 6, device="cuda")
+  back[:10, 2] = 2.0 ** torch.arange(10, 0, -1, device="cuda") - 1.0
+  assert torch.equal(dx[:, 0], back) and torch.equal(dstate[0], torch.tensor([0, 0, 2.0 * 1023, 0, 0, 0], device="cuda"))
+  assert not dgate[:10].any() and not dgate[:, :, 2:].any()
+
+
 def test_saturated_gates():
   """Infinite and lowest-value gates keep or replace the state exactly."""
   lowest = torch.finfo(BF16).min
@@ -455,6 +472,19 @@ def test_other_stream():
   for a, b in zip(got, want):
     assert torch.equal(a, b)
   assert torch.equal(y, seqops.dropout(args[0], 0.5, 1))
+
+
+def test_step_in_place_is_seen_by_autograd():
+  """A state that autograd has saved and a step overwrites is not used for a gradient."""
+  state, w = rnd(3, 8, seed=1), rnd(3, 8, seed=2).requires_grad_()
+  loss = (w * state).sum()
+  with torch.no_grad():
+    seqops.gated_step(rnd(3, 8, seed=3), rnd(3, 8, seed=4), state, out=state)
+  with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+    loss.backward()
+  with torch.inference_mode():
+    h, new = seqops.gated_step(rnd(3, 8, seed=3), rnd(3, 8, seed=4), state, out=torch.empty_like(state))
+  assert new.is_inference()
 
 
 def test_gpu_refusals():

@@ -53,6 +53,17 @@ def test_gradients_reach_every_parameter_and_differ_by_dropout():
   assert int(mem.dropout_step) == 2 and torch.equal(a, b)
 
 
+def test_state_made_in_inference_mode_serves_outside():
+  mem = PolicyMemory(7, dim=12).eval()
+  obs = torch.randn(3, 7)
+  with torch.inference_mode():
+    first = mem.step(obs).clone()
+  mem.reset_state(3)
+  assert torch.equal(mem.step(obs), first)
+  feats, _ = mem(obs[None], mem.state.clone())
+  feats.sum().backward()
+
+
 def test_refusals():
   for kw in (dict(num_gates=5), dict(num_layers=0), dict(dropout=1.0), dict(num_gates=0)):
     with pytest.raises(ValueError):

@@ -101,6 +101,13 @@ def test_dropout_gradient_keeps_the_mask():
   assert torch.equal(g != 0, y != 0) and torch.equal(g[g != 0], torch.full_like(g[g != 0], 2.0))
 
 
+def test_last_state_of_no_steps_is_a_copy():
+  state = torch.ones(2, 4)
+  _, last = seqops.gated_scan(torch.zeros(0, 2, 4), torch.zeros(0, 2, 4), state)
+  last.zero_()
+  assert state.all()
+
+
 def test_empty_calls():
   for t, n, d in ((0, 2, 3), (4, 0, 3), (4, 2, 0)):
     h, last = seqops.gated_scan(torch.zeros(t, n, d), torch.zeros(t, n, d), torch.ones(n, d))
