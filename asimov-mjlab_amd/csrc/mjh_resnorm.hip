@@ -6,10 +6,12 @@
 //   n = norm_pre(s)
 // The statistics, s inside n, and all sums are float32; s and n are rounded once, at their store.
 //
-// Rows of up to 2,048 elements (16-bit types: 4,096): a group of lanes holds a row, 8 elements a lane, so every tensor is read once and every
-// statistic is taken from registers (the variance around the mean, in a second pass over registers). 8 to 64 lanes,
-// several rows a workgroup, or a workgroup of two to eight waves. Longer rows: streams over the row, which read it
-// again, largely from the caches, where holding it would leave a CU one workgroup and nothing to hide its barriers.
+// Rows of up to 2,048 elements (16-bit types: 4,096; forward also float32 rows of up to 4,096 that fill their waves,
+// 2,047 x 4,096: 39 us, 49 as streams): a group of lanes holds a row, 8 elements a lane, so every tensor is read once
+// and every statistic is taken from registers (the variance around the mean, in a second pass over registers). One lane
+// (rows shorter than 16 bytes) to 64, several rows a workgroup, or a workgroup of two to eight waves. Longer rows:
+// streams over the row, which read it again, largely from the caches, where holding it would leave a CU one workgroup
+// and nothing to hide its barriers (2,048 x 8,192 bfloat16, forward: 57 us, 63 held by 16 waves).
 // The backward pass keeps s and p nowhere: it forms them again from y, residual and gate, the tensors that it has to
 // read in any case, with the forward pass's (mean, rstd) of each row. Weight gradients: a group (a thread that owns
 // columns) adds its rows in registers, groups of a workgroup join in shared memory, workgroups in a second launch,
@@ -61,6 +63,7 @@ __device__ __forceinline__ float dpp(float v) {
 }
 template <int L>
 __device__ __forceinline__ float lane_sum(float v) {
+  if (L == 1) return v;
   v += dpp<0xB1>(v);                 // quad_perm 1 0 3 2
   v += dpp<0x4E>(v);                 // quad_perm 2 3 0 1
   v += dpp<0x141>(v);                // row_half_mirror
@@ -70,26 +73,36 @@ __device__ __forceinline__ float lane_sum(float v) {
   return v;
 }
 
-// Where a lane's N neighbouring elements of a row lie: slot p holds elements p N and on; what is left of a row that N
-// does not divide lies one element a slot behind them, so that no lane goes through a piece element by element.
-// FULL: every slot is a whole piece.
-template <class T, int N, bool FULL>
+// Where a lane's N neighbouring elements of a row lie: slot p holds elements p N and on. What is left of a row that N
+// does not divide (kTail) is the end of the row's last N elements, of which the slot's own are marked: every lane reads
+// whole pieces and none in a branch, whose result would be waited for there (98,304 x 99 floats, backward: 75 us, 96
+// with a branch for single elements).
+// kWhole: every slot is a piece of its own. kTiny: rows shorter than a piece, slot 0 reads them element by element.
+enum { kWhole, kTail, kTiny };
+template <class T, int N, int FIT>
 struct Piece {
-  int c, cnt;  // first column; N, 1 or 0 columns
+  static constexpr unsigned kAll = (1u << N) - 1u;
+  int c;          // first column read
+  unsigned mask;  // bit j: element c + j is the slot's own
   __device__ __forceinline__ Piece() {}
-  __device__ __forceinline__ Piece(int p, int D) {
-    const int whole = D / N, left = D - whole * N;
-    c = p < whole ? p * N : whole * N + (p - whole);
-    cnt = FULL || p < whole ? N : p < whole + left ? 1 : 0;
+  __device__ __forceinline__ Piece(int p, int D) : c(p * N), mask(kAll) {
+    if (FIT == kTail) {
+      c = min(c, D - N);
+      const int skip = p * N - c;
+      mask = skip >= N ? 0u : kAll << skip & kAll;
+    } else if (FIT == kTiny) {
+      c = 0;
+      mask = p ? 0u : (1u << D) - 1u;
+    }
   }
-  __device__ __forceinline__ bool has(int j) const { return FULL || j < cnt; }
+  __device__ __forceinline__ bool has(int j) const { return FIT == kWhole || (mask >> j & 1u); }
   template <class W>
   __device__ __forceinline__ Pack<W, N> get(const W* q) const {
+    if constexpr (FIT != kTiny) return load_loose<W, N>(q + c);
     Pack<W, N> v{};
-    if (FULL || cnt == N)
-      v = load_loose<W, N>(q + c);
-    else if (cnt)
-      v.v[0] = q[c];
+#pragma unroll
+    for (int j = 0; j < N; j++)
+      if (has(j)) v.v[j] = q[j];
     return v;
   }
   __device__ __forceinline__ Pack<T, N> read(const void* p, ll row, ll step) const {
@@ -97,10 +110,13 @@ struct Piece {
   }
   __device__ __forceinline__ void write(void* p, ll row, ll step, const float (&f)[N]) const {
     T* q = static_cast<T*>(p) + row * step + c;
-    if (FULL || cnt == N)
+    if (FIT == kWhole || mask == kAll) {
       store_loose<T, N>(q, f);
-    else if (cnt)
-      *q = (T)f[0];
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; j++)
+        if (has(j)) q[j] = (T)f[j];
+    }
   }
   // channel weights; `none` where there are none
   __device__ __forceinline__ void weights(const void* w, int w32, float none, float* o) const {
@@ -125,11 +141,12 @@ struct Piece {
   }
   // keep bits (bit j: element j). Neighbours share a word, and the words of a piece are one addition apart; a piece
   // that begins at an odd index begins with the second half of a word.
+  template <bool EVEN>  // D and c are even
   __device__ __forceinline__ unsigned keep_bits(unsigned long long base, const Drop& d, ll row, int D) const {
     const unsigned long long i = (unsigned long long)(row * D + c);
     unsigned long long z = base + ((i >> 1) + 1ull) * 0x9e3779b97f4a7c15ull, w = mjh::mix64(z);
     unsigned bits = 0;
-    const bool odd = !FULL && (i & 1);
+    const bool odd = !EVEN && (i & 1);
     if (odd) bits = drop_keep(w, 1, d.thr);
 #pragma unroll
     for (int j = 0; j < N; j += 2) {
@@ -188,7 +205,7 @@ __device__ __forceinline__ void activate(const T (&g)[N], const Args& a, float (
 }
 
 // ---- rows held in registers -------------------------------------------------------------
-// TPR: 8 to 64 lanes hold a row; 256, 512: a workgroup of a.tpr threads (whole waves) does.
+// TPR: 1 (rows shorter than a piece), or 8 to 64 lanes hold a row; 256, 512: a workgroup of a.tpr threads (whole waves) does.
 constexpr int threads_of(int tpr) { return tpr > 256 ? tpr : 256; }
 template <class T, bool FULL, int TPR>
 struct Row {
@@ -196,13 +213,14 @@ struct Row {
   static constexpr bool kWaves = TPR > 64;
   static constexpr int kGroups = kWaves ? 1 : 256 / TPR;  // rows a workgroup holds
   int group, lane, lanes, D, turn = 0;
-  Piece<T, N, FULL> at[kPieces];
+  typedef Piece<T, N, (FULL ? kWhole : TPR == 1 ? kTiny : kTail)> At;
+  At at[kPieces];
   __device__ __forceinline__ explicit Row(const Args& a) : D(a.D) {
     lanes = kWaves ? a.tpr : TPR;
     lane = kWaves ? threadIdx.x : threadIdx.x % TPR;
     group = kWaves ? 0 : threadIdx.x / TPR;
 #pragma unroll
-    for (int k = 0; k < kPieces; k++) at[k] = Piece<T, N, FULL>(k * lanes + lane, a.D);
+    for (int k = 0; k < kPieces; k++) at[k] = At(k * lanes + lane, a.D);
   }
   __device__ __forceinline__ bool has(int k) const { return at[k / N].has(k % N); }
   __device__ __forceinline__ void read(const void* p, ll row, ll step, bool on, T (&o)[kPer]) const {
@@ -235,7 +253,7 @@ struct Row {
   __device__ __forceinline__ unsigned keep_bits(unsigned long long base, const Drop& d, ll row) const {
     unsigned bits = 0;
 #pragma unroll
-    for (int k = 0; k < kPieces; k++) bits |= (at[k].keep_bits(base, d, row, D) & ((1u << N) - 1u)) << (k * N);
+    for (int k = 0; k < kPieces; k++) bits |= (at[k].template keep_bits<FULL>(base, d, row, D) & ((1u << N) - 1u)) << (k * N);
     return bits;
   }
   // Sums of NV values over a row's lanes, in every lane. Several waves: through shared memory (2 x 8 x 2 floats), in
@@ -261,14 +279,14 @@ struct Row {
           for (int k = 0; k < NV; k++) v[k] += s[j * 2 + k];
     }
   }
-  // mean and 1 / deviation of a row held in registers (columns that are not there hold 0 in v)
+  // mean and 1 / deviation of a row held in registers
   __device__ __forceinline__ void stats(const float (&v)[kPer], const Args& a, float (*shared)[16], float& mean, float& rstd) {
     mean = 0.f;
     float t[1];
     if (a.layer) {
       t[0] = 0.f;
 #pragma unroll
-      for (int k = 0; k < kPer; k++) t[0] += v[k];
+      for (int k = 0; k < kPer; k++) t[0] += has(k) ? v[k] : 0.f;
       sum<1>(t, shared);
       mean = t[0] * a.inv;
     }
@@ -297,8 +315,6 @@ __global__ __launch_bounds__(threads_of(TPR)) void resnorm_forward(const Args a)
   at.weights(a.pre_w, a.w32, 1.f, pre_w);
   at.weights(a.pre_b, a.w32, 0.f, pre_b);
   at.scales(a, scale);
-  // No row is held while another is worked on: the waves that its registers cost hide more (65,536 x 300 bfloat16: 102 us against 125,
-  // 98,304 x 256: 56 against 57).
   T raw[kPer], raw_y[kPer], raw_g[kPer];
   auto fetch = [&](ll row) {
     const bool on = row < a.R;
@@ -334,9 +350,6 @@ __global__ __launch_bounds__(threads_of(TPR)) void resnorm_forward(const Args a)
       at.write(a.s, row, a.ss, on, s);
     }
     if (a.pre) {
-#pragma unroll
-      for (int k = 0; k < kPer; k++)
-        if (!at.has(k)) s[k] = 0.f;
       at.stats(s, a, shared, pre_mean, pre_rstd);
 #pragma unroll
       for (int k = 0; k < kPer; k++) s[k] = __builtin_fmaf((s[k] - pre_mean) * pre_rstd, pre_w[k], pre_b[k]);
@@ -526,21 +539,21 @@ struct Block256 {
 struct Moments {
   float n = 0.f, mean = 0.f, m2 = 0.f;
   template <int N>
-  __device__ __forceinline__ void add(const float (&v)[N], int cnt, int layer) {
+  __device__ __forceinline__ void add(const float (&v)[N], unsigned mask, int layer) {
     if (!layer) {
 #pragma unroll
       for (int j = 0; j < N; j++)
-        if (j < cnt) m2 += v[j] * v[j];
+        if (mask >> j & 1u) m2 += v[j] * v[j];
       return;
     }
-    if (!cnt) return;
-    const float k = (float)cnt, inv = cnt == N ? 1.f / N : 1.f;
+    if (!mask) return;
+    const float k = (float)__popc(mask), inv = __builtin_amdgcn_rcpf(k);
     float m = 0.f, q = 0.f;
 #pragma unroll
-    for (int j = 0; j < N; j++) m += j < cnt ? v[j] : 0.f;
+    for (int j = 0; j < N; j++) m += mask >> j & 1u ? v[j] : 0.f;
     m *= inv;
 #pragma unroll
-    for (int j = 0; j < N; j++) q += j < cnt ? (v[j] - m) * (v[j] - m) : 0.f;
+    for (int j = 0; j < N; j++) q += mask >> j & 1u ? (v[j] - m) * (v[j] - m) : 0.f;
     const float share = k * __builtin_amdgcn_rcpf(n + k), d = m - mean;
     m2 += q + d * d * n * share;
     mean += d * share;
@@ -557,6 +570,16 @@ struct Moments {
   }
 };
 
+// f(piece, slot) over a row's slots by a workgroup of 256; the row's end, where it is no whole piece, in a call of its
+// own, so that the others need no masks (2,048 x 8,192 bfloat16: 63 us, 78 with them).
+template <class T, int N, class F>
+__device__ __forceinline__ void over_row(int D, F f) {
+  const int whole = D / N;
+#pragma unroll 2
+  for (int p = threadIdx.x; p < whole; p += 256) f(Piece<T, N, kWhole>(p, D), p);
+  if (D % N && (int)threadIdx.x == whole % 256) f(Piece<T, N, kTail>(whole, D), whole);
+}
+
 // One workgroup a row, three passes over it: the statistics of y; s, which is written, and its statistics; n. The
 // float32 s waits in shared memory for the last pass (KEEP, up to 8,192 columns, each thread's own), or is formed once
 // more: n is not taken from the rounded s.
@@ -569,23 +592,21 @@ __global__ __launch_bounds__(256) void resnorm_stream(const Args a) {
   const ll row = a.row0 + blockIdx.x;
   const bool block = a.y != nullptr;
   const unsigned long long base = a.drop.thr ? drop_base(a.drop) : 0;
-  const int slots = a.D / N + a.D % N;
+  const int slots = (a.D + N - 1) / N;
   Block256 b;
   float mean = 0.f, rstd = 1.f, pre_mean = 0.f, pre_rstd = 1.f;
   if (block && a.post) {
     Moments m;
-#pragma unroll 2
-    for (int p = threadIdx.x; p < slots; p += 256) {
-      const Piece<T, N, false> at(p, a.D);
+    over_row<T, N>(a.D, [&](const auto& at, int) {
       const auto y = at.read(a.y, row, a.ys);
       float v[N];
 #pragma unroll
       for (int j = 0; j < N; j++) v[j] = (float)y.v[j];
-      m.add(v, at.cnt, a.layer);
-    }
+      m.add(v, at.mask, a.layer);
+    });
     m.finish(a, b, shared, mean, rstd);
   }
-  auto form = [&](const Piece<T, N, false>& at, float (&s)[N]) {
+  auto form = [&](const auto& at, float (&s)[N]) {
     const auto r = at.read(a.r, row, a.rs);
 #pragma unroll
     for (int j = 0; j < N; j++) s[j] = (float)r.v[j];
@@ -603,7 +624,7 @@ __global__ __launch_bounds__(256) void resnorm_stream(const Args a) {
       for (int j = 0; j < N; j++) p[j] = __builtin_fmaf((p[j] - mean) * rstd, w[j], bias[j]);
     }
     if (a.drop.thr) {
-      const unsigned keep = at.keep_bits(base, a.drop, row, a.D);
+      const unsigned keep = at.template keep_bits<false>(base, a.drop, row, a.D);
 #pragma unroll
       for (int j = 0; j < N; j++) p[j] = (keep >> j & 1u) ? p[j] * a.drop.scale : 0.f;
     }
@@ -614,24 +635,20 @@ __global__ __launch_bounds__(256) void resnorm_stream(const Args a) {
   };
   Moments m;
   if (block || a.pre) {
-#pragma unroll 2
-    for (int p = threadIdx.x; p < slots; p += 256) {
-      const Piece<T, N, false> at(p, a.D);
+    over_row<T, N>(a.D, [&](const auto& at, int p) {
       float s[N];
       form(at, s);
       if (block) at.write(a.s, row, a.ss, s);
-      m.add(s, at.cnt, a.layer);
+      m.add(s, at.mask, a.layer);
       if (KEEP) {
 #pragma unroll
         for (int j = 0; j < N; j++) kept[j * slots + p] = s[j];
       }
-    }
+    });
   }
   if (a.pre) {
     m.finish(a, b, shared, pre_mean, pre_rstd);
-#pragma unroll 2
-    for (int p = threadIdx.x; p < slots; p += 256) {
-      const Piece<T, N, false> at(p, a.D);
+    over_row<T, N>(a.D, [&](const auto& at, int p) {
       float s[N], w[N], bias[N];
       if (KEEP) {
 #pragma unroll
@@ -644,7 +661,7 @@ __global__ __launch_bounds__(256) void resnorm_stream(const Args a) {
 #pragma unroll
       for (int j = 0; j < N; j++) s[j] = __builtin_fmaf((s[j] - pre_mean) * pre_rstd, w[j], bias[j]);
       at.write(a.n, row, a.ns, s);
-    }
+    });
   }
   if (a.stats && threadIdx.x == 0) store<float, 4>(a.stats + row * 4, {mean, rstd, pre_mean, pre_rstd});
 }
@@ -656,16 +673,13 @@ __global__ __launch_bounds__(256) void resnorm_stream(const Args a) {
 // in them, ds = X - rstd (hat c0 + c1) with X = ds_in + rstd dn w, so the first stream takes the sums of X q, hat q
 // and q (q = the factor from ds to the gradient of the normalised y, once times yhat, once alone) in the same pass.
 // 4 elements a thread, whatever the type: 8 of a 16-bit type cost the registers of half the waves (2,048 x 8,192
-// bfloat16: 104 us against 72).
+// bfloat16: 104 us, then 72 as 4).
 constexpr int kBack = 4;
-template <class T>
-using BackPiece = Piece<T, kBack, false>;
-
 template <class T>
 struct Raw {
   Pack<T, kBack> y, r, g, ds, dn;
-  template <bool BLOCK>
-  __device__ __forceinline__ void fetch(const Args& a, const BackPiece<T>& at, ll row) {
+  template <bool BLOCK, class P>
+  __device__ __forceinline__ void fetch(const Args& a, const P& at, ll row) {
     if (BLOCK) {
       y = at.read(a.y, row, a.ys);
       if (a.gate) g = at.read(a.gate, row, a.gs);
@@ -684,7 +698,8 @@ struct Formed {
   static constexpr int N = kBack;
   float ds[N], dn[N], hat[N], yhat[N], u[N], av[N], slope[N];
   unsigned keep;
-  __device__ __forceinline__ Formed(const Args& a, const BackPiece<T>& at, const Raw<T>& raw, const Pack<float, 4>& st, ll row,
+  template <class P>
+  __device__ __forceinline__ Formed(const Args& a, const P& at, const Raw<T>& raw, const Pack<float, 4>& st, ll row,
                                     unsigned long long base, const float (&post_w)[N], const float (&post_b)[N],
                                     const float (&scale)[N]) {
     keep = ~0u;
@@ -702,7 +717,7 @@ struct Formed {
         u[j] = a.post ? (BIAS ? __builtin_fmaf(yhat[j], post_w[j], post_b[j]) : yhat[j] * post_w[j]) : yhat[j];
       }
       if (a.drop.thr) {
-        keep = at.keep_bits(base, a.drop, row, a.D);
+        keep = at.template keep_bits<false>(base, a.drop, row, a.D);
 #pragma unroll
         for (int j = 0; j < N; j++) u[j] = (keep >> j & 1u) ? u[j] * a.drop.scale : 0.f;
       }
@@ -726,10 +741,8 @@ __global__ __launch_bounds__(256) void resnorm_rows(const Args a) {
   const ll row = a.row0 + blockIdx.x;
   const unsigned long long base = BLOCK && a.drop.thr ? drop_base(a.drop) : 0;
   const auto st = load<float, 4>(a.stats + row * 4);
-  const int slots = a.D / N + a.D % N;
   float t[8] = {};  // dv hat, dv, X q0, hat q0, q0, X q1, hat q1, q1
-  for (int p = threadIdx.x; p < slots; p += 256) {
-    const BackPiece<T> at(p, a.D);
+  over_row<T, N>(a.D, [&](const auto& at, int) {
     Raw<T> raw;
     raw.template fetch<BLOCK>(a, at, row);
     float pre_w[N], post_w[N], post_b[N], scale[N];
@@ -759,7 +772,7 @@ __global__ __launch_bounds__(256) void resnorm_rows(const Args a) {
         t[7] += q;
       }
     }
-  }
+  });
 #pragma unroll
   for (int k = 0; k < 8; k++) {
     t[k] = lane_sum<64>(t[k]);
@@ -779,8 +792,8 @@ __global__ __launch_bounds__(256) void resnorm_rows(const Args a) {
 template <class T, bool BLOCK, bool BIAS>
 __global__ __launch_bounds__(64) void resnorm_columns(const Args a) {
   constexpr int N = kBack;
-  const BackPiece<T> at(blockIdx.x * 64 + threadIdx.x, a.D);
-  if (!at.cnt) return;
+  const Piece<T, N, kTail> at(blockIdx.x * 64 + threadIdx.x, a.D);
+  if (!at.mask) return;
   const unsigned long long base = BLOCK && a.drop.thr ? drop_base(a.drop) : 0;
   float pre_w[N], post_w[N], post_b[N], scale[N];
   at.weights(a.pre_w, a.w32, 1.f, pre_w);
@@ -949,9 +962,10 @@ __global__ __launch_bounds__(256) void dropout_rows(const DropArgs a) {
 }
 
 // ---- host side ------------------------------------------------------------------------
-// lanes that hold a row (8 elements each, as slots of 16 bytes): a power of two up to a wave, then whole waves
+// lanes that hold a row (8 elements each, as slots of 16 bytes): one, a power of two up to a wave, then whole waves
 int lanes_of(int D, int dtype) {
-  const int n = dtype == MJH_F32 ? 4 : 8, slots = D / n + D % n, lanes = (slots * n + kPer - 1) / kPer;
+  const int n = dtype == MJH_F32 ? 4 : 8, slots = (D + n - 1) / n, lanes = (slots * n + kPer - 1) / kPer;
+  if (D < n) return 1;
   if (lanes > 64) return (lanes + 63) / 64 * 64;
   int t = 8;
   while (t < lanes) t *= 2;
@@ -962,7 +976,7 @@ bool long_row(int D, int dtype) { return lanes_of(D, dtype) > (dtype == MJH_F32 
 // the backward pass's parts write partial sums each, so a part takes several rows
 unsigned parts_of(int D, ll rows, int dtype) {
   if (long_row(D, dtype)) {
-    const ll tiles = (D / kBack + D % kBack + 63) / 64;
+    const ll tiles = ((D + kBack - 1) / kBack + 63) / 64;
     return (unsigned)std::max<ll>(1, std::min<ll>(rows / 4, kColumnWaves / tiles));
   }
   const int lanes = lanes_of(D, dtype);
@@ -1011,37 +1025,48 @@ Args args_of(const mjh_resnorm_desc& d) {
 
 bool wants_bias(const mjh_resnorm_desc& d) { return d.post_b || d.pre_b; }
 
+// As many workgroups as are resident, each with the same number of row groups: one more round of a few workgroups, or
+// one more row for some, costs what a whole round does (forward, 8,191 x 2,999 bfloat16: 116 us, 149 with 32 waves a CU
+// asked for whatever their registers).
+template <class K>
+int waves_per_simd(K kernel) {
+  int n = 0;
+  return hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, 256, 0) == hipSuccess && n ? n : 2;
+}
+ll resident(int threads, int waves_simd) { return 256ll * std::max(1, waves_simd * 256 / threads); }
 template <class T, bool FULL, int TPR>
 void launch_forward(const Args& a, hipStream_t s) {
-  const ll groups = TPR > 64 ? 1 : 256 / TPR, waves = TPR > 64 ? a.tpr / 64 : 4;
-  const ll need = (a.R + groups - 1) / groups;
-  resnorm_forward<T, FULL, TPR><<<dim3((unsigned)std::min<ll>(need, 256 * 32 / waves)), dim3(TPR > 64 ? a.tpr : 256), 0, s>>>(a);
+  static const int waves_simd = waves_per_simd(resnorm_forward<T, FULL, TPR>);
+  const int threads = TPR > 64 ? a.tpr : 256;
+  const ll per = TPR > 64 ? 1 : 256 / TPR, groups = (a.R + per - 1) / per, most = resident(threads, waves_simd);
+  const ll rounds = (groups + most - 1) / most, grid = (groups + rounds - 1) / rounds;
+  resnorm_forward<T, FULL, TPR><<<dim3((unsigned)grid), dim3(threads), 0, s>>>(a);
 }
-// As many parts as are resident, where the rows are enough: a part takes the same share of the rows, so one more round
-// of a few workgroups costs a whole round (98,304 x 99 floats, 2 waves a SIMD by their registers: 93 us as 2 workgroups
-// a CU, 119 as 3; 98,304 x 256 bfloat16, 3 waves a SIMD: 99 and 86). At most parts_of(), which the workspace holds.
+// As many parts as are resident, where the rows are enough (98,304 x 99 floats, 2 waves a SIMD by their registers: 94
+// us as 2 workgroups a CU, 119 as 3; 98,304 x 256 bfloat16, 3 waves a SIMD: 99 and 86). Each has sums to write and join, so a part
+// takes 4 rows at least (parts_of(), which the workspace holds).
 template <class T, bool FULL, int TPR, bool BLOCK, bool BIAS>
 void launch_backward(Args& a, hipStream_t s) {
-  static const int waves_simd = [] {
-    int n = 0;
-    const bool ok = hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, resnorm_backward<T, FULL, TPR, BLOCK, BIAS>, 256, 0) == hipSuccess;
-    return ok && n ? n : 2;
-  }();
+  static const int waves_simd = waves_per_simd(resnorm_backward<T, FULL, TPR, BLOCK, BIAS>);
   const int threads = TPR > 64 ? a.tpr : 256;
-  a.parts = std::min(a.parts, 256 * std::max(1, waves_simd * 256 / threads));
+  a.parts = (int)std::min<ll>(a.parts, resident(threads, waves_simd));
   resnorm_backward<T, FULL, TPR, BLOCK, BIAS><<<dim3(a.parts), dim3(threads), 0, s>>>(a);
 }
 template <class T, bool FULL>
 void launch_forward_rows(const Args& a, hipStream_t s) {
+  if constexpr (!FULL)
+    if (a.tpr == 1) return launch_forward<T, FULL, 1>(a, s);
   if (a.tpr == 8) return launch_forward<T, FULL, 8>(a, s);
   if (a.tpr == 16) return launch_forward<T, FULL, 16>(a, s);
   if (a.tpr == 32) return launch_forward<T, FULL, 32>(a, s);
   if (a.tpr == 64) return launch_forward<T, FULL, 64>(a, s);
-  if (sizeof(T) == 4 || a.tpr <= 256) return launch_forward<T, FULL, 256>(a, s);
-  if constexpr (sizeof(T) == 2) launch_forward<T, FULL, 512>(a, s);
+  if (a.tpr <= 256) return launch_forward<T, FULL, 256>(a, s);
+  if constexpr (sizeof(T) == 2 || FULL) launch_forward<T, FULL, 512>(a, s);
 }
 template <class T, bool FULL, bool BLOCK, bool BIAS>
 void launch_backward_rows(Args& a, hipStream_t s) {
+  if constexpr (!FULL)
+    if (a.tpr == 1) return launch_backward<T, FULL, 1, BLOCK, BIAS>(a, s);
   if (a.tpr == 8) return launch_backward<T, FULL, 8, BLOCK, BIAS>(a, s);
   if (a.tpr == 16) return launch_backward<T, FULL, 16, BLOCK, BIAS>(a, s);
   if (a.tpr == 32) return launch_backward<T, FULL, 32, BLOCK, BIAS>(a, s);
@@ -1059,7 +1084,7 @@ template <class T, bool BLOCK, bool BIAS>
 void launch_backward_as(Args& a, bool streams, hipStream_t s) {
   if (streams) {
     by_row(a, [&](const Args& b, unsigned rows) { resnorm_rows<T, BLOCK, BIAS><<<dim3(rows), dim3(256), 0, s>>>(b); });
-    resnorm_columns<T, BLOCK, BIAS><<<dim3((a.D / kBack + a.D % kBack + 63) / 64, a.parts), dim3(64), 0, s>>>(a);
+    resnorm_columns<T, BLOCK, BIAS><<<dim3(((a.D + kBack - 1) / kBack + 63) / 64, a.parts), dim3(64), 0, s>>>(a);
   } else if (a.tpr * kPer == a.D) {
     launch_backward_rows<T, true, BLOCK, BIAS>(a, s);
   } else {
@@ -1073,9 +1098,11 @@ void launch_type(const mjh_resnorm_desc& d, Args& a, bool back, hipStream_t s) {
     bias ? launch_backward_as<T, true, true>(a, streams, s) : launch_backward_as<T, true, false>(a, streams, s);
   else if (back)
     bias ? launch_backward_as<T, false, true>(a, streams, s) : launch_backward_as<T, false, false>(a, streams, s);
+  else if (streams && a.tpr <= 512 && a.tpr * kPer == a.D)
+    launch_forward_rows<T, true>(a, s);
   else if (streams && a.D <= 8192)
     by_row(a, [&](const Args& b, unsigned rows) {
-      resnorm_stream<T, true><<<dim3(rows), dim3(256), 4 * (16 / sizeof(T)) * (a.D / (16 / sizeof(T)) + a.D % (16 / sizeof(T))), s>>>(b);
+      resnorm_stream<T, true><<<dim3(rows), dim3(256), a.D * 4 + 64, s>>>(b);
     });
   else if (streams)
     by_row(a, [&](const Args& b, unsigned rows) { resnorm_stream<T, false><<<dim3(rows), dim3(256), 0, s>>>(b); });

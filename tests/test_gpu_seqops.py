@@ -281,6 +281,23 @@ def test_residual_norm(r, d, dtype, wtype, norm):
              ctr=torch.tensor([5], device="cuda") if d > 99 else None)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("r,d", [(1030, 1), (1030, 3), (700, 4), (300, 5), (300, 7), (300, 8), (130, 9), (61, 15), (33, 65),
+                                 (9, 511), (9, 513), (3, 4093), (3, 4095), (3, 4103), (5, 8197)])
+def test_residual_norm_row_ends(r, d, dtype):
+  """Rows shorter than a load, as long as one, and just before and behind the sizes where a row's holder changes; rows of a
+  wider tensor, whose neighbours hold NaN that no row may pick up."""
+  v, ds, dn = norm_inputs(r, d, dtype, F32, bias=True)
+  wide = torch.full((r, d + 3), float("nan"), device="cuda", dtype=dtype)
+  for name in ("y", "res", "gate"):
+    rows = wide.clone()[:, 1 : d + 1]
+    rows.copy_(v[name])
+    v[name] = rows
+  check_norm(v, ds, dn, "layer", p=0.25)
+  v["post_b"] = v["pre_b"] = None
+  check_norm(v, ds, dn, "rms", p=0.25)
+
+
 @pytest.mark.parametrize("post", [False, True])
 @pytest.mark.parametrize("pre", [False, True])
 @pytest.mark.parametrize("gated,scaled,bias", [(False, 0, False), (True, 0, True), (False, 2, False), (True, 1, False)])
