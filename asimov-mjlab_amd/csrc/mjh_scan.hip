@@ -257,8 +257,10 @@ __device__ __forceinline__ int wave_max(int v) {
   return __builtin_amdgcn_readfirstlane(v);
 }
 
-// What a chunk's steps do to the state that comes in, h -> A h + B: A = product of a, B = the result from 0. Bound by
-// the card's rate of reading (16,384 x 2,048 bfloat16: 24 us, 2.9 TB/s; 1 to 4 blocks of loads under way are the same).
+// What a chunk's steps do to the state that comes in, h -> A h + B: A = product of a, B = the result from 0. One
+// reading of x and gate (16,384 x 2,048 bfloat16: 16 us, 4.3 TB/s; 23 within a training pass, after a launch whose
+// outputs are still being written out; more loads under way, or wider ones, are the same). 64 registers, so that all
+// 524,288 threads are resident.
 template <class T, class GT, int V, int GV, bool BLEND>
 __global__ __launch_bounds__(kBlock, 8) void scan_forward_agg(const Args a) {
   const Where w = flat_where<V>(a);
