@@ -118,9 +118,10 @@ struct Gate {
 // The chunks' results become the state that comes into each chunk (forward: from the chunks before it; BACK: the
 // gradient from the chunks after it), written over the chunk's own result in agg_b. A workgroup holds 32 channels
 // by up to 32 groups; a group takes kJoin neighbouring chunks, all loads in flight at once (2,048 channels by 512
-// chunks: 8.3 us; 16 channels by 64 groups 9.3, 8 by 64 14; one thread a channel and a loop over 256 chunks 70). A
+// chunks: 6.8 us; 16 channels by 64 groups 1 more, 8 by 64 6 more; one thread a channel and a loop over 256 chunks 70). A
 // chunk with a reset inside passes nothing on, whatever comes in (not 0 times it: the state before a reset may be
-// infinite or NaN), and a state of 0 adds nothing, however far the product of the gates overflows.
+// infinite or NaN), and a state of 0 adds nothing, however far the product of the gates overflows. No load stands in a
+// branch, where it would be waited for (1,000 x 8 x 99 with resets: 4.7 us, 9.7 with its flags' loads in one).
 constexpr int kJoin = 16, kMaxChunks = 32 * kJoin;
 __device__ __forceinline__ float carry(float p, float s, float q, bool cut) {
   return cut || s == 0.f ? q : __builtin_fmaf(p, s, q);
@@ -130,21 +131,35 @@ __global__ __launch_bounds__(1024) void scan_join(const Args a) {
   __shared__ float sa[32][32], sb[32][32];
   __shared__ unsigned char sc[32][32];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const ll nd = (ll)a.N * a.D, at = (ll)blockIdx.x * 32 + lane;
-  const bool on = at < nd;
-  const int n = on ? (int)(at / a.D) : 0;
+  const ll nd = (ll)a.N * a.D, own = (ll)blockIdx.x * 32 + lane, at = min(own, nd - 1);
+  const bool on = own < nd;
+  const int n = (int)((unsigned)at / (unsigned)a.D);
   const float* edge = BACK ? a.dlast : a.state;
   const float first = on && edge ? edge[at] : 0.f;
   float p[kJoin], q[kJoin];
   bool cut[kJoin];
+  unsigned flag[kJoin];
+#pragma unroll
+  for (int k = 0; k < kJoin; k++) {  // chunks behind the last read the last again: a load in a branch is waited for there
+    const int i = min(w * kJoin + k, a.nchunk - 1);  // in the order of the recurrence
+    const ll c = BACK ? a.nchunk - 1 - i : i;
+    p[k] = a.agg_a[c * nd + at];
+    q[k] = a.agg_b[c * nd + at];
+    flag[k] = 0;
+  }
+  if (a.reset) {
+#pragma unroll
+    for (int k = 0; k < kJoin; k++) {
+      const int i = min(w * kJoin + k, a.nchunk - 1);
+      flag[k] = a.agg_cut[(ll)(BACK ? a.nchunk - 1 - i : i) * a.N + n];
+    }
+  }
 #pragma unroll
   for (int k = 0; k < kJoin; k++) {
-    const int i = w * kJoin + k;  // in the order of the recurrence
-    const bool in = on && i < a.nchunk;
-    const int c = in ? (BACK ? a.nchunk - 1 - i : i) : 0;
-    p[k] = in ? a.agg_a[c * nd + at] : 1.f;
-    q[k] = in ? a.agg_b[c * nd + at] : 0.f;
-    cut[k] = in && a.reset && a.agg_cut[(ll)c * a.N + n];
+    const bool in = w * kJoin + k < a.nchunk;
+    p[k] = in ? p[k] : 1.f;
+    q[k] = in ? q[k] : 0.f;
+    cut[k] = in && flag[k];
   }
   float ta = 1.f, tb = 0.f;
   bool tc = false;
@@ -654,8 +669,16 @@ bool fits(const mjh_scan_desc& s, int v) {
   return true;
 }
 
+// Two neighbouring channels a thread where strides allow (16,384 x 2,048 bfloat16, shared gates: 133 us of kernels
+// against 153 with one; 24 x 8,192 x 512: 367, 388), but for gates of their own in 65,536 to 131,072 channels, which one
+// channel a thread makes enough threads for a launch without chunks (200 x 480 x 256: 134 us, 148 in chunks).
+//
+// Chunks: from kFull threads on none (24 x 4,096 x 256: 99 us). Below, enough for kThreads threads, of kLeast blocks of
+// steps each (16,384 x 2,048: 133 us, 138 for half as many threads, 132 for twice; 4,001 x 12 x 512: 47, 50, 47), or of
+// one block while that makes no more than kFew threads (1,000 x 8 x 99: 30 us, 38 without; for all, 200 x 240 x 256: 99
+// against 93).
 constexpr int kWide = 2;
-constexpr ll kThreads = 524288, kFull = 65536, kLeast = 2;
+constexpr ll kThreads = 524288, kFull = 65536, kLeast = 2, kFew = 262144;
 
 int make_plan(const mjh_scan_desc* s, Plan& p) {
   if (!s) return refuse("scan: no description");
@@ -681,12 +704,15 @@ int make_plan(const mjh_scan_desc* s, Plan& p) {
   a.dstate = s->dstate;
   a.T = s->T; a.N = s->N; a.D = s->D; a.G = s->G; a.K = s->D / s->G;
   p.heads = a.K > 1;
-  set_width(p, fits(*s, kWide) ? kWide : 1);
-  // chunks: enough threads to keep the card's loads in flight, each chunk some blocks of steps long
+  const ll channels = (ll)a.N * a.D;
+  set_width(p, fits(*s, kWide) && (p.heads || channels < kFull || channels >= kWide * kFull) ? kWide : 1);
   const ll threads = (ll)a.N * a.dv;
   const ll blocks = (a.T + kSteps - 1) / kSteps;
-  ll n = threads >= kFull ? 1 : (kThreads + threads - 1) / threads;
-  n = std::max<ll>(1, std::min<ll>(std::min<ll>(n, blocks / kLeast), kMaxChunks));
+  ll n = 1;
+  if (threads < kFull) {
+    n = std::max(std::min((kThreads + threads - 1) / threads, blocks / kLeast), std::min(kFew / threads, blocks));
+    n = std::max<ll>(1, std::min<ll>(n, kMaxChunks));
+  }
   const ll per_chunk = (blocks + n - 1) / n;
   a.chunk = (int)(per_chunk * kSteps);
   a.nchunk = (int)((a.T + a.chunk - 1) / a.chunk);

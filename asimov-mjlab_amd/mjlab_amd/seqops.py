@@ -90,8 +90,8 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor | None =
 
   The gradients of x, gate and state start from the float32 states, not from the rounded h. The
   backward pass needs ``ceil(T / 8) N D`` kept float32 values. Time: one pass over the tensors; with
-  fewer than 65,536 channels (times 2 where neighbours are read in pairs) in N D, x, gate and the
-  gradient of h are read a second time, by the launch that forms the chunks' effects."""
+  few channels (N D below 65,536; 131,072 for shared gates) and many steps, x, gate and the gradient
+  of h are read a second time, by the launch that forms the chunks' effects."""
   out = (_EXT or _ext()).gated_scan(x, gate, state, reset, lengths, _MODES.get(mode, -1))
   return _scan_torch(x, gate, state, reset, lengths, mode) if out is None else out
 
