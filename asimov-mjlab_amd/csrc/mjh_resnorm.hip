@@ -893,6 +893,7 @@ template <class T>
 __global__ __launch_bounds__(256) void resnorm_join_scale(const Join j) {
   __shared__ float part[256];
   float t = 0.f;
+#pragma unroll 8
   for (int c = threadIdx.x; c < j.D; c += 256) t += j.scale_cols[c];
   part[threadIdx.x] = t;
   __syncthreads();

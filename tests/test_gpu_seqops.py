@@ -78,6 +78,40 @@ def test_scan_in_chunks(t, n, d, g, dtype, gtype, mode):
     check_scan(scan_inputs(t, n, d, g, mode, dtype, gtype, resets, ragged, rows_first), mode)
 
 
+@pytest.mark.parametrize("t,n,d,g,dtype", [(t, 3, 10, 10, F32) for t in (15, 16, 17, 31, 33, 100)] + [
+  (20, 300, 256, 256, BF16), (40, 300, 256, 4, F16), (70, 200, 256, 256, BF16), (8200, 1, 2, 1, F32)])
+def test_scan_plans(t, n, d, g, dtype):
+  """Chunks of one block and their ends, one and two channels a thread, the most chunks there are."""
+  check_scan(scan_inputs(t, n, d, g, "blend", dtype, dtype, resets=0.03, ragged=True), "blend")
+
+
+def test_scan_lengths_below_zero_are_zero():
+  args = list(scan_inputs(300, 4, 12, 12, "decay", F32, F32))
+  args[4] = torch.tensor([-5, 0, -(2**31), 300], dtype=torch.int32, device="cuda")
+  got = run_scan(*args, "decay")
+  args[4] = args[4].clamp(min=0)
+  for a, b in zip(got, check_scan(args, "decay")):
+    assert torch.equal(a, b)
+
+
+def test_one_tensor_in_several_places():
+  """Gradients of a tensor that is input and gate, or branch, residual and gate, add up."""
+  x = rnd(40, 3, 16, seed=1)
+  leaf = x.clone().requires_grad_()
+  h, last = seqops.gated_scan(leaf, leaf)
+  (got,) = torch.autograd.grad([h, last], leaf, [torch.ones_like(h), torch.ones_like(last)])
+  parts = run_scan(x, x, torch.zeros(3, 16, device="cuda"), None, None, torch.ones_like(h), torch.ones_like(last), "blend")
+  assert torch.equal(got, parts[2] + parts[3])
+  w, v = torch.ones(16, device="cuda"), x[:, 0].clone().requires_grad_()
+  s, n = seqops.residual_norm(v, v, pre_weight=w, post_weight=w, gate=v)
+  (got,) = torch.autograd.grad([s, n], v, [x[:, 1], x[:, 2]])
+  leaves = [x[:, 0].clone().requires_grad_() for _ in range(3)]
+  s, n = seqops.residual_norm(leaves[0], leaves[1], pre_weight=w, post_weight=w, gate=leaves[2])
+  parts = torch.autograd.grad([s, n], leaves, [x[:, 1], x[:, 2]])
+  total = sum(p.double() for p in parts)  # float32 additions in whatever order: two roundings of at most 3 terms
+  assert ((got.double() - total).abs() <= 3 * seq_ref.U * sum(p.double().abs() for p in parts)).all()
+
+
 def test_scan_rows_with_nothing():
   """Rows of length zero, rows cleared at every step, and lengths beyond the last step."""
   x, gate, state, _, _, dh, dl = scan_inputs(300, 5, 20, 20, "blend", BF16, BF16)
@@ -489,6 +523,42 @@ def test_other_stream():
   for a, b in zip(got, want):
     assert torch.equal(a, b)
   assert torch.equal(y, seqops.dropout(args[0], 0.5, 1))
+
+
+def test_threads_at_once():
+  """Four threads with streams of their own: forward and backward passes of several shapes, as each alone."""
+  import threading
+
+  jobs = [scan_inputs(400 + 50 * i, 2, 40 + 8 * i, 40 + 8 * i, "blend", BF16, BF16, resets=0.02, seed=i) for i in range(4)]
+  w = [1 + rnd(72, seed=31 + i, scale=0.1) for i in range(2)]
+
+  def work(i):
+    h = run_scan(*jobs[i], "blend")
+    d = h[0].shape[-1]
+    leaf = h[0].detach().requires_grad_()
+    s, n = seqops.residual_norm(leaf, leaf.detach(), pre_weight=w[0][:d], post_weight=w[1][:d], p=0.1, seed=i)
+    return [*h, s.detach(), n.detach(), *torch.autograd.grad(n, leaf, jobs[i][5])]
+
+  want = [work(i) for i in range(4)]
+  torch.cuda.synchronize()
+  wrong = []
+
+  def run(i):
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+      for _ in range(5):
+        got = work(i)
+        side.synchronize()
+        wrong.extend((i, k) for k, (a, b) in enumerate(zip(got, want[i])) if not torch.equal(a, b))
+    done.append(i)
+
+  done = []
+  threads = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+  for th in threads:
+    th.start()
+  for th in threads:
+    th.join()
+  assert sorted(done) == [0, 1, 2, 3] and not wrong, wrong
 
 
 def test_step_in_place_is_seen_by_autograd():
