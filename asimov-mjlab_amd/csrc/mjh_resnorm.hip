@@ -571,11 +571,12 @@ struct Moments {
 };
 
 // f(piece, slot) over a row's slots by a workgroup of 256; the row's end, where it is no whole piece, in a call of its
-// own, so that the others need no masks (2,048 x 8,192 bfloat16: 63 us, 78 with them).
+// own, so that the others need no masks (2,048 x 8,192 bfloat16, forward: 63 us, 78 with them). One piece at a time:
+// the waves are many (backward's row sums, 2,047 x 4,097 floats: 31 us, 33 by twos, 42 by fours).
 template <class T, int N, class F>
 __device__ __forceinline__ void over_row(int D, F f) {
   const int whole = D / N;
-#pragma unroll 2
+#pragma unroll 1
   for (int p = threadIdx.x; p < whole; p += 256) f(Piece<T, N, kWhole>(p, D), p);
   if (D % N && (int)threadIdx.x == whole % 256) f(Piece<T, N, kTail>(whole, D), whole);
 }

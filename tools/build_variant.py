@@ -21,15 +21,19 @@ name, flags = sys.argv[1], sys.argv[2:]
 OUTD.mkdir(parents=True, exist_ok=True)
 tmp = Path("/tmp/mjh_variants") / name
 tmp.mkdir(parents=True, exist_ok=True)
-srcs = [CSRC / f for f in ("mjh_step.hip", "mjh_envops.hip", "mjh_mdp.hip", "mjh_mgr.hip", "mjh_fuse.hip", "mjh_scan.hip",
-                           "mjh_resnorm.hip")]
+srcs = [CSRC / f for f in ("mjh_step.hip", "mjh_envops.hip", "mjh_mdp.hip", "mjh_mgr.hip", "mjh_fuse.hip")]
+objs = []
+for f in ("mjh_scan.hip", "mjh_resnorm.hip"):  # with the flags of their own that the library has them built with
+  objs.append(tmp / (f + ".o"))
+  subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", f"-I{ROOT / 'include'}", "-Xclang",
+                  "-target-feature", "-Xclang", "-packed-fp32-ops", "-c", "-o", str(objs[-1]), str(CSRC / f)], check=True)
 if os.environ.get("MJH_STEP_SRC"):  # A/B against another revision of the step kernel (e.g. a saved HEAD copy)
   srcs[0] = Path(os.environ["MJH_STEP_SRC"])
 
 
 def hipcc(table: Path, out: Path) -> None:
   cmd = ["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", f"-I{ROOT / 'include'}", f"-I{CSRC}",
-         f'-DMJH_SPEC_TABLE="{table}"', *flags, "-o", str(out), *map(str, srcs)]
+         f'-DMJH_SPEC_TABLE="{table}"', *flags, "-o", str(out), *map(str, srcs), *(f"-Wl,{o}" for o in objs)]
   subprocess.run(cmd, check=True)
 
 
