@@ -205,7 +205,8 @@ __device__ __forceinline__ void activate(const T (&g)[N], const Args& a, float (
 }
 
 // ---- rows held in registers -------------------------------------------------------------
-// TPR: 1 (rows shorter than a piece), or 8 to 64 lanes hold a row; 256, 512: a workgroup of a.tpr threads (whole waves) does.
+// TPR: 1 (rows shorter than a piece), or 8 to 64 lanes hold a row; 256, 512: a workgroup of a.tpr threads (whole
+// waves) does.
 constexpr int threads_of(int tpr) { return tpr > 256 ? tpr : 256; }
 template <class T, bool FULL, int TPR>
 struct Row {
@@ -300,8 +301,8 @@ struct Row {
   }
 };
 
-// Bound by bytes (98,304 x 256 bfloat16, all parts: 54 us, 4.7 TB/s; 16,384 x 2,048: 49 us, 5.5 TB/s); for a few rows by
-// its chain of sums (16 x 1,000 float16: 4.5 us).
+// Bound by bytes (98,304 x 256 bfloat16, all parts: 54 us, 4.7 TB/s; 16,384 x 2,048: 49 us, 5.5 TB/s); for a few rows
+// by its chain of sums (16 x 1,000 float16: 4.5 us).
 template <class T, bool FULL, int TPR>
 __global__ __launch_bounds__(threads_of(TPR)) void resnorm_forward(const Args a) {
   typedef Row<T, FULL, TPR> R;
@@ -1048,8 +1049,8 @@ void launch_forward(const Args& a, hipStream_t s) {
   resnorm_forward<T, FULL, TPR><<<dim3((unsigned)grid), dim3(threads), 0, s>>>(a);
 }
 // As many parts as are resident, where the rows are enough (98,304 x 99 floats, 2 waves a SIMD by their registers: 94
-// us as 2 workgroups a CU, 119 as 3; 98,304 x 256 bfloat16, 3 waves a SIMD: 99 and 86). Each has sums to write and join, so a part
-// takes 4 rows at least (parts_of(), which the workspace holds).
+// us as 2 workgroups a CU, 119 as 3; 98,304 x 256 bfloat16, 3 waves a SIMD: 99 and 86). Each has sums to write and
+// join, so a part takes 4 rows at least (parts_of(), which the workspace holds).
 template <class T, bool FULL, int TPR, bool BLOCK, bool BIAS>
 void launch_backward(Args& a, hipStream_t s) {
   static const int waves_simd = waves_per_simd(resnorm_backward<T, FULL, TPR, BLOCK, BIAS>);

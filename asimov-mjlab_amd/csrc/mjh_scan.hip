@@ -118,10 +118,10 @@ struct Gate {
 // The chunks' results become the state that comes into each chunk (forward: from the chunks before it; BACK: the
 // gradient from the chunks after it), written over the chunk's own result in agg_b. A workgroup holds 32 channels
 // by up to 32 groups; a group takes kJoin neighbouring chunks, all loads in flight at once (2,048 channels by 512
-// chunks: 6.8 us; 16 channels by 64 groups 1 more, 8 by 64 6 more; one thread a channel and a loop over 256 chunks 70). A
-// chunk with a reset inside passes nothing on, whatever comes in (not 0 times it: the state before a reset may be
-// infinite or NaN), and a state of 0 adds nothing, however far the product of the gates overflows. No load stands in a
-// branch, where it would be waited for (1,000 x 8 x 99 with resets: 4.7 us, 9.7 with its flags' loads in one).
+// chunks: 6.8 us; 16 channels by 64 groups 1 more, 8 by 64 6 more; one thread a channel and a loop over 256 chunks
+// 70). A chunk with a reset inside passes nothing on, whatever comes in (not 0 times it: the state before a reset may
+// be infinite or NaN), and a state of 0 adds nothing, however far the product of the gates overflows. No load stands
+// in a branch, where it would be waited for (1,000 x 8 x 99 with resets: 4.7 us, 9.7 with its flags' loads in one).
 constexpr int kJoin = 16, kMaxChunks = 32 * kJoin;
 __device__ __forceinline__ float carry(float p, float s, float q, bool cut) {
   return cut || s == 0.f ? q : __builtin_fmaf(p, s, q);
@@ -140,7 +140,7 @@ __global__ __launch_bounds__(1024) void scan_join(const Args a) {
   bool cut[kJoin];
   unsigned flag[kJoin];
 #pragma unroll
-  for (int k = 0; k < kJoin; k++) {  // chunks behind the last read the last again: a load in a branch is waited for there
+  for (int k = 0; k < kJoin; k++) {  // chunks behind the last read the last again
     const int i = min(w * kJoin + k, a.nchunk - 1);  // in the order of the recurrence
     const ll c = BACK ? a.nchunk - 1 - i : i;
     p[k] = a.agg_a[c * nd + at];
@@ -324,9 +324,9 @@ __global__ __launch_bounds__(kBlock, 8) void scan_forward_agg(const Args a) {
   if (a.reset && w.d == 0) a.agg_cut[(ll)c * a.N + w.n] = cut;
 }
 
-// The outputs. Bound by bytes (24 x 4,096 x 256 bfloat16 with kept states: 38 us, 4.4 TB/s). AHEAD: loads of the next block under way while this one is worked on, for chunked launches; with a
-// thread for every channel of many rows the waves that its registers cost are worth more (24 x 4,096 x 256 bfloat16:
-// 33 us against 40).
+// The outputs. Bound by bytes (24 x 4,096 x 256 bfloat16 with kept states: 38 us, 4.4 TB/s). AHEAD: loads of the next
+// block under way while this one is worked on, for chunked launches; with a thread for every channel of many rows the
+// waves that its registers cost are worth more (24 x 4,096 x 256 bfloat16 without kept states: 33 us against 40).
 template <class T, class GT, int V, int GV, bool BLEND, bool AHEAD>
 __global__ __launch_bounds__(kBlock) void scan_forward(const Args a) {
   const Where w = flat_where<V>(a);
@@ -602,7 +602,8 @@ __global__ __launch_bounds__(kBlock) void scan_join_heads(const Args a) {
   static_cast<GT*>(a.dgate)[(tn / a.N) * a.dgt + (tn % a.N) * a.dgn + g] = (GT)sum;
 }
 
-// One step (4,096 x 256 bfloat16: 4.1 us, 3.6 TB/s; 1 x 128: 1.4 us): out = a h' + ..., the state read from a.state and written to a.last (the same rows, or others).
+// One step: out = a h' + ..., the state read from a.state and written to a.last (the same rows, or others). 4,096 x 256
+// bfloat16: 4.1 us, 3.6 TB/s; 1 x 128: 1.4 us.
 template <class T, class GT, int V, int GV, bool BLEND>
 __global__ __launch_bounds__(kBlock) void scan_step(const Args a) {
   const Where w = flat_where<V>(a);
