@@ -813,10 +813,13 @@ __global__ __launch_bounds__(64) void resnorm_columns(const Args a) {
 #pragma unroll
     for (int j = 0; j < N; j++) sum[q][j] = 0.f;
   Raw<T> cur, next;
+  auto st = load<float, 4>(a.stats + (ll)blockIdx.y * 4), k = load<float, 4>(a.coef + (ll)blockIdx.y * 4);
   cur.template fetch<BLOCK>(a, at, blockIdx.y);
+  wait_loads();
   for (ll row = blockIdx.y; row < a.R; row += gridDim.y) {
-    if (row + gridDim.y < a.R) next.template fetch<BLOCK>(a, at, row + gridDim.y);
-    const auto st = load<float, 4>(a.stats + row * 4), k = load<float, 4>(a.coef + row * 4);
+    const ll ahead = min(row + gridDim.y, (ll)a.R - 1);  // under way while this row is worked on
+    const auto next_st = load<float, 4>(a.stats + ahead * 4), next_k = load<float, 4>(a.coef + ahead * 4);
+    next.template fetch<BLOCK>(a, at, ahead);
     const Formed<T, BLOCK, BIAS> f(a, at, cur, st, row, base, post_w, post_b, scale);
     float ds[N], dg[N];
 #pragma unroll
@@ -846,6 +849,8 @@ __global__ __launch_bounds__(64) void resnorm_columns(const Args a) {
       if (a.dy) at.write(a.dy, row, a.dys, ds);
     }
     cur = next;
+    st = next_st;
+    k = next_k;
   }
   if (!a.sums) return;
   float* out = a.sums + (ll)blockIdx.y * kSums * a.D;

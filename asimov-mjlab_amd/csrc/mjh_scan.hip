@@ -340,6 +340,7 @@ __global__ __launch_bounds__(kBlock) void scan_forward(const Args a) {
   T* ph = static_cast<T*>(a.h) + (ll)w.n * a.hn + w.d;
   Block<T, GT, V, GV, true, false> b, next;
   if (AHEAD && t0 < stop) b.read(a, w, flags, t0 < live, t0, t1);
+  if (AHEAD) wait_loads();
   int tb = t0;
   for (; tb < stop; tb += kSteps) {
     if (a.kept && w.on) store<float, V>(a.kept + (ll)(tb / kSteps) * nd + at, s);
@@ -487,6 +488,7 @@ __global__ __launch_bounds__(kBlock) void scan_backward(const Args a) {
     if (tb < live) tok = load<float, V>(a.kept + (ll)(tb / kSteps) * nd + at);
   };
   fetch(b, k, last);
+  wait_loads();
   for (int tb = last; tb >= t0; tb -= kSteps) {
     fetch(next, nextk, tb - kSteps);  // under way while this block is worked on
     float sum[kSteps];
