@@ -14,7 +14,6 @@ Operators
 
 from __future__ import annotations
 
-import functools
 import math
 import sys
 from pathlib import Path
@@ -32,10 +31,10 @@ M64 = (1 << 64) - 1
 NORM_EPS = 1e-5
 
 
-@functools.cache
 def _seqops():
-  """The framework's operators, imported once as a program does (not looked up at every call)."""
-  sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "asimov-mjlab_amd"))
+  pkg = str(Path(__file__).resolve().parents[1] / "asimov-mjlab_amd")
+  if pkg not in sys.path:
+    sys.path.insert(0, pkg)
   from mjlab_amd import seqops
 
   return seqops
