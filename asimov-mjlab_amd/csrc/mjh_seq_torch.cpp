@@ -83,6 +83,13 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
     if (t->defined() && t->requires_grad()) return true;
   return false;
 }
+// Kernels have no forward-mode derivatives: a tangent would be lost without a word. (Where forward mode is off, as inside
+// a torch.autograd.Function with a jvp of its own, only the values are wanted.)
+void no_tangent(const char* name, std::initializer_list<const Tensor*> ts) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* t : ts)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), name, ": no forward-mode derivatives on the GPU (use reverse mode)");
+}
 Tensor workspace(ll bytes, const char* what, const Tensor& like) {
   TORCH_CHECK(bytes >= 0, what, " refused: ", lib.last_error());
   return bytes ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor();
@@ -197,6 +204,7 @@ struct Scan : torch::autograd::Function<Scan> {
     const auto saved = ctx->get_saved_variables();
     variable_list out(6);
     if (!grads[0].defined() && !grads[1].defined()) return out;
+    no_tangent("gated_scan's backward pass", {&grads[0], &grads[1]});
     c10::DeviceGuard guard(saved[0].device());
     const Tensor x = unit(saved[0]), gate = unit(saved[1]), reset = saved[2];
     const Tensor lengths = saved[3].defined() ? saved[3].contiguous() : saved[3];
@@ -234,6 +242,7 @@ py::object gated_scan(const Tensor& x, const Tensor& gate, const Maybe& state_, 
   const Tensor state = or_none(state_), reset = or_none(reset_), lengths = or_none(lengths_);
   check_scan("gated_scan", x, gate, state, reset, lengths, mode, 3);
   if (!x.is_cuda() || x.numel() == 0) return py::none();
+  no_tangent("gated_scan", {&x, &gate, &state});
   if (wants_grad({&x, &gate, &state})) {
     auto o = Scan::apply(x, gate, maybe(state), maybe(reset), maybe(lengths), (int64_t)mode);
     return py::make_tuple(std::move(o[0]), std::move(o[1]));
@@ -274,6 +283,7 @@ py::object gated_step(const Tensor& x0, const Tensor& gate0, const Maybe& state_
     if (overlap(out, x0) || overlap(out, gate0) || (reset.defined() && overlap(out, reset))) refuse(name, ": out overlaps an input");
   }
   if (!x0.is_cuda() || x0.numel() == 0) return py::none();
+  no_tangent(name, {&x0, &gate0, &state, &out});
   c10::DeviceGuard guard(x0.device());
   if (!out.defined()) out = at::empty(state.sizes(), state.options());
   if (!state.is_contiguous()) state = state.contiguous();
@@ -348,6 +358,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list out(6);
     if (!grads[0].defined()) return out;
+    no_tangent("dropout's backward pass", {&grads[0]});
     const auto v = ctx->saved_data["stream"].toIntVector();
     const Stream r{(unsigned long long)v[0], (unsigned long long)v[1], (unsigned long long)v[2]};
     out[0] = dropout_run(grads[0], ctx->saved_data["scale"].toDouble(), r, ctx->get_saved_variables()[0], Tensor());
@@ -362,6 +373,7 @@ py::object dropout(const Tensor& x, double p, unsigned long long seed, unsigned 
   known_device("dropout", x);
   const Stream r = check_drop("dropout", p, seed, key, ctr, x);
   if (!x.is_cuda() || x.numel() == 0) return py::none();
+  no_tangent("dropout", {&x});
   const double scale = scale_.has_value() ? *scale_ : drop_scale(p);
   if (wants_grad({&x})) return py::cast(Dropout::apply(x, scale, (int64_t)r.thr, (int64_t)r.seed, (int64_t)r.key, maybe(ctr)));
   return py::cast(dropout_run(x, scale, r, ctr, Tensor()));
@@ -497,6 +509,7 @@ struct Resnorm : torch::autograd::Function<Resnorm> {
     if (a.y.t.defined()) ds0 = grads[k++];
     if (a.pre_w.defined()) dn0 = grads[k++];
     if (!ds0.defined() && !dn0.defined()) return out;
+    no_tangent("residual_norm's backward pass", {&ds0, &dn0});
     c10::DeviceGuard guard(a.r.t.device());
     const Rows ds(ds0), dn(dn0);
     const Norm o = Norm::unpack(ctx->saved_data["options"].toIntVector());
@@ -561,6 +574,7 @@ py::object residual_norm(const Maybe& y_, const Tensor& r, const Maybe& pre_w_,
   if (!y.defined()) o.r.thr = 0;
   if (!r.is_cuda() || r.numel() == 0) return py::none();
   if (dim > 1 << 24 || r.numel() / dim > 0x7fffffff) refuse(name, ": at most 2^31 rows of at most 2^24 elements, got ", r.sizes());
+  no_tangent(name, {&y, &r, &gate, &w[0], &w[1], &w[2], &w[3], &w[4]});
   Tensor s = r, n;
   if (wants_grad({&y, &r, &gate, &w[0], &w[1], &w[2], &w[3], &w[4]})) {
     auto out = Resnorm::apply(maybe(y), maybe(r), maybe(gate), maybe(w[0]), maybe(w[1]), maybe(w[2]), maybe(w[3]), maybe(w[4]), maybe(ctr),

@@ -4,7 +4,8 @@ dropout whose mask is never stored. GPU tensors run the HIP kernels through the 
 ``mjlab_amd._seqops`` (csrc/mjh_seq_torch.cpp: checks, allocation, autograd nodes; there is no torch
 fallback there, what a kernel does not take is refused); CPU tensors, which only the CPU test
 harness uses, take the torch formulas below, which are the semantics. All three differentiate
-through ``torch.autograd`` (once), run on the current stream of the tensors' device, allocate
+through ``torch.autograd`` (once, in reverse mode; the kernels have no forward-mode derivatives, and
+an operand or incoming gradient that carries a tangent is refused on the GPU), run on the current stream of the tensors' device, allocate
 through torch's caching allocator only and can be captured into a graph. Two calls never share a
 workspace.
 

@@ -1,0 +1,35 @@
+"""Policy-memory operators on the CPU at the limits of what their entry points take."""
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd
+
+from mjlab_amd import seqops
+
+
+def rnd(*shape, seed=0):
+  return torch.randn(*shape, generator=torch.Generator().manual_seed(seed))
+
+
+CALLS = {
+  "gated_scan": (lambda *v: seqops.gated_scan(*v)[0], ((5, 2, 8), (5, 2, 4), (2, 8))),
+  "dropout": (lambda v: seqops.dropout(v, 0.5, 1), ((5, 8),)),
+  "residual_norm": (lambda y, r, g, w: sum(seqops.residual_norm(y, r, gate=g, post_weight=w, pre_weight=w)), ((5, 8),) * 3 + ((8,),)),
+}
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_forward_mode_on_the_cpu(name):
+  """The torch formulas carry a tangent: <up, J tangent> is <J^T up, tangent> of reverse mode."""
+  call, shapes = CALLS[name]
+  args = [rnd(*s, seed=i) for i, s in enumerate(shapes)]
+  tangents = [rnd(*s, seed=10 + i) for i, s in enumerate(shapes)]
+  with fwd.dual_level():
+    out = fwd.unpack_dual(call(*(fwd.make_dual(a, t) for a, t in zip(args, tangents))))
+  up = rnd(*out.primal.shape, seed=20)
+  grads = torch.autograd.grad(call(*(a.requires_grad_() for a in args)), args, up)
+  a = (out.tangent.double() * up).sum()
+  terms = [(g.double() * t) for g, t in zip(grads, tangents)]
+  # two float32 evaluations of at most 80 outputs, each of some 20 roundings, terms of size up to about 10
+  assert abs(a - sum(t.sum() for t in terms)) <= 40 * 2.0**-24 * 10 * (sum(t.abs().sum() for t in terms) + 80)
+  assert float(a.abs()) > 1e-3
