@@ -47,7 +47,7 @@ struct Args {
   void* dx; ll dxt, dxn;
   void* dgate; ll dgt, dgn;
   float* dstate;
-  float* agg_a; float* agg_b; unsigned char* agg_cut;  // per chunk: (N, D), (N, D), (N,)
+  double* agg_a; float* agg_b; unsigned char* agg_cut;  // per chunk: (N, D), (N, D), (N,)
   float* part;                                         // per-wave sums of a head wider than a wave: (T, N, G, W)
   int T, N, D, G, K;  // K = D / G channels per gate
   int dv;             // vectors per row
@@ -118,17 +118,23 @@ struct Gate {
 // The chunks' results become the state that comes into each chunk (forward: from the chunks before it; BACK: the
 // gradient from the chunks after it), written over the chunk's own result in agg_b. A workgroup holds 32 channels
 // by up to 32 groups; a group takes kJoin neighbouring chunks, all loads in flight at once (2,048 channels by 512
-// chunks: 6.8 us; 16 channels by 64 groups 1 more, 8 by 64 6 more; one thread a channel and a loop over 256 chunks
+// chunks: 8.3 us; 16 channels by 64 groups 1 more, 8 by 64 6 more; one thread a channel and a loop over 256 chunks
 // 70). A chunk with a reset inside passes nothing on, whatever comes in (not 0 times it: the state before a reset may
 // be infinite or NaN), and a state of 0 adds nothing, however far the product of the gates overflows. No load stands
-// in a branch, where it would be waited for (1,000 x 8 x 99 with resets: 4.7 us, 9.7 with its flags' loads in one).
+// in a branch, where it would be waited for (1,000 x 8 x 99 with resets: 5.0 us, twice that with its flags' loads in one).
+//
+// Products of gates are float64, here and in the launches that form them: a small state may grow, and a large one
+// shrink, by any factor of up to 2^277 inside float32's range, over a chunk or a group of them. A product beyond
+// float64's range takes every other state beyond float32's in either case: the recurrence itself overflows there
+// (a product of infinity and a later 0 is its NaN too) or has nothing left. 1.6 us of the 8.3.
 constexpr int kJoin = 16, kMaxChunks = 32 * kJoin;
-__device__ __forceinline__ float carry(float p, float s, float q, bool cut) {
-  return cut || s == 0.f ? q : __builtin_fmaf(p, s, q);
+__device__ __forceinline__ float carry(double p, float s, float q, bool cut) {
+  return cut || s == 0.f ? q : (float)__builtin_fma(p, (double)s, (double)q);
 }
 template <bool BACK>
 __global__ __launch_bounds__(1024) void scan_join(const Args a) {
-  __shared__ float sa[32][32], sb[32][32];
+  __shared__ double sa[32][32];
+  __shared__ float sb[32][32];
   __shared__ unsigned char sc[32][32];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const ll nd = (ll)a.N * a.D, own = (ll)blockIdx.x * 32 + lane, at = min(own, nd - 1);
@@ -136,9 +142,9 @@ __global__ __launch_bounds__(1024) void scan_join(const Args a) {
   const int n = (int)((unsigned)at / (unsigned)a.D);
   const float* edge = BACK ? a.dlast : a.state;
   const float first = on && edge ? edge[at] : 0.f;
-  float p[kJoin], q[kJoin];
-  bool cut[kJoin];
-  unsigned flag[kJoin];
+  double p[kJoin];
+  float q[kJoin];
+  unsigned flag[kJoin], cut = 0;  // cut, bit k: a reset inside chunk k
 #pragma unroll
   for (int k = 0; k < kJoin; k++) {  // chunks behind the last read the last again
     const int i = min(w * kJoin + k, a.nchunk - 1);  // in the order of the recurrence
@@ -157,21 +163,20 @@ __global__ __launch_bounds__(1024) void scan_join(const Args a) {
 #pragma unroll
   for (int k = 0; k < kJoin; k++) {
     const bool in = w * kJoin + k < a.nchunk;
-    p[k] = in ? p[k] : 1.f;
+    p[k] = in ? p[k] : 1.;
     q[k] = in ? q[k] : 0.f;
-    cut[k] = in && flag[k];
+    cut |= (unsigned)(in && flag[k]) << k;
   }
-  float ta = 1.f, tb = 0.f;
-  bool tc = false;
+  double ta = 1.;
+  float tb = 0.f;
 #pragma unroll
   for (int k = 0; k < kJoin; k++) {
-    tb = carry(p[k], tb, q[k], cut[k]);
+    tb = carry(p[k], tb, q[k], cut >> k & 1u);
     ta *= p[k];
-    tc |= cut[k];
   }
   sa[w][lane] = ta;
   sb[w][lane] = tb;
-  sc[w][lane] = tc;
+  sc[w][lane] = cut != 0;
   __syncthreads();
   float s = first;
 #pragma unroll 8
@@ -181,7 +186,7 @@ __global__ __launch_bounds__(1024) void scan_join(const Args a) {
     const int i = w * kJoin + k;
     if (!on || i >= a.nchunk) break;
     a.agg_b[(BACK ? a.nchunk - 1 - i : i) * nd + at] = s;
-    s = carry(p[k], s, q[k], cut[k]);
+    s = carry(p[k], s, q[k], cut >> k & 1u);
   }
 }
 
@@ -272,21 +277,31 @@ __device__ __forceinline__ int wave_max(int v) {
   return __builtin_amdgcn_readfirstlane(v);
 }
 
+template <int V>
+__device__ __forceinline__ void store_products(double* p, const double (&f)[V]) {
+  Pack<double, V> o;
+#pragma unroll
+  for (int v = 0; v < V; v++) o.v[v] = f[v];
+  *reinterpret_cast<Pack<double, V>*>(p) = o;
+}
+
 // What a chunk's steps do to the state that comes in, h -> A h + B: A = product of a, B = the result from 0. One
 // reading of x and gate (16,384 x 2,048 bfloat16: 16 us, 4.3 TB/s; 23 within a training pass, after a launch whose
 // outputs are still being written out; more loads under way, or wider ones, are the same). 64 registers, so that all
-// 524,288 threads are resident.
+// 524,288 threads are resident; 72 for two gates a thread, which spill in 64 (200 x 240 x 256 blend, backward: 15.0 us,
+// 16.2 so).
 template <class T, class GT, int V, int GV, bool BLEND>
-__global__ __launch_bounds__(kBlock, 8) void scan_forward_agg(const Args a) {
+__global__ __launch_bounds__(kBlock, GV == 2 ? 7 : 8) void scan_forward_agg(const Args a) {
   const Where w = flat_where<V>(a);
   const Flags flags(w);
   const int c = blockIdx.y, t0 = c * a.chunk, t1 = min(a.T, t0 + a.chunk);
   const int live = !w.on ? 0 : a.lengths ? min(a.lengths[w.n], t1) : t1;
   const int stop = a.lengths ? wave_max(live) : t1;  // the same in all lanes, as every read and ballot needs
   const ll nd = (ll)a.N * a.D, at = (ll)w.n * a.D + w.d;
-  float s[V], prod[V];
+  float s[V];
+  double prod[V];
 #pragma unroll
-  for (int v = 0; v < V; v++) s[v] = 0.f, prod[v] = 1.f;
+  for (int v = 0; v < V; v++) s[v] = 0.f, prod[v] = 1.;
   bool cut = false;
   for (int tb = t0; tb < stop; tb += kSteps) {
     Block<T, GT, V, GV, true, false> b;
@@ -300,7 +315,7 @@ __global__ __launch_bounds__(kBlock, 8) void scan_forward_agg(const Args a) {
           const Gate<BLEND> f((float)b.g[j].v[GV == 1 ? 0 : v]);
           const float x = (float)b.x[j].v[v];
           s[v] = __builtin_fmaf(f.a, s[v], BLEND ? f.b * x : x);
-          prod[v] *= f.a;
+          prod[v] *= (double)f.a;
         }
     } else {
 #pragma unroll
@@ -313,13 +328,13 @@ __global__ __launch_bounds__(kBlock, 8) void scan_forward_agg(const Args a) {
           const Gate<BLEND> f((float)b.g[j].v[GV == 1 ? 0 : v]);
           const float x = (float)b.x[j].v[v];
           s[v] = __builtin_fmaf(f.a, reset ? 0.f : s[v], BLEND ? f.b * x : x);
-          prod[v] = reset ? 0.f : prod[v] * f.a;
+          prod[v] = reset ? 0. : prod[v] * (double)f.a;
         }
       }
     }
   }
   if (!w.on) return;
-  store<float, V>(a.agg_a + c * nd + at, prod);
+  store_products(a.agg_a + c * nd + at, prod);
   store<float, V>(a.agg_b + c * nd + at, s);
   if (a.reset && w.d == 0) a.agg_cut[(ll)c * a.N + w.n] = cut;
 }
@@ -389,16 +404,17 @@ __global__ __launch_bounds__(kBlock) void scan_forward(const Args a) {
 
 // The chunk's effect on the gradient that comes in from the steps after it.
 template <class T, class GT, int V, int GV, bool BLEND>
-__global__ __launch_bounds__(kBlock, 8) void scan_backward_agg(const Args a) {
+__global__ __launch_bounds__(kBlock, GV == 2 ? 7 : 8) void scan_backward_agg(const Args a) {
   const Where w = flat_where<V>(a);
   const Flags flags(w);
   const int c = blockIdx.y, t0 = c * a.chunk, t1 = min(a.T, t0 + a.chunk);
   const int live = !w.on ? 0 : a.lengths ? min(a.lengths[w.n], t1) : t1;
   const int stop = a.lengths ? wave_max(live) : t1;
   const ll nd = (ll)a.N * a.D, at = (ll)w.n * a.D + w.d;
-  float e[V], prod[V];
+  float e[V];
+  double prod[V];
 #pragma unroll
-  for (int v = 0; v < V; v++) e[v] = 0.f, prod[v] = 1.f;
+  for (int v = 0; v < V; v++) e[v] = 0.f, prod[v] = 1.;
   bool cut = false;
   for (int tb = t0 + (max(stop - t0, 0) + kSteps - 1) / kSteps * kSteps - kSteps; tb >= t0; tb -= kSteps) {
     Block<T, GT, V, GV, false, true> b;
@@ -411,7 +427,7 @@ __global__ __launch_bounds__(kBlock, 8) void scan_backward_agg(const Args a) {
         for (int v = 0; v < V; v++) {
           const Gate<BLEND> f((float)b.g[j].v[GV == 1 ? 0 : v]);
           e[v] = f.a * ((float)b.dh[j].v[v] + e[v]);
-          prod[v] *= f.a;
+          prod[v] *= (double)f.a;
         }
     } else {
 #pragma unroll
@@ -423,13 +439,13 @@ __global__ __launch_bounds__(kBlock, 8) void scan_backward_agg(const Args a) {
         for (int v = 0; v < V; v++) {
           const Gate<BLEND> f((float)b.g[j].v[GV == 1 ? 0 : v]);
           e[v] = reset ? 0.f : f.a * ((float)b.dh[j].v[v] + e[v]);
-          prod[v] = reset ? 0.f : prod[v] * f.a;
+          prod[v] = reset ? 0. : prod[v] * (double)f.a;
         }
       }
     }
   }
   if (!w.on) return;
-  store<float, V>(a.agg_a + c * nd + at, prod);
+  store_products(a.agg_a + c * nd + at, prod);
   store<float, V>(a.agg_b + c * nd + at, e);
   if (a.reset && w.d == 0) a.agg_cut[(ll)c * a.N + w.n] = cut;
 }
@@ -728,7 +744,7 @@ ll agg_floats(const Plan& p) {
   const Args& a = p.a;
   if (a.nchunk == 1) return 0;
   const ll nd = (ll)a.N * a.D;
-  return 2 * a.nchunk * nd + ((ll)a.nchunk * a.N + 3) / 4;
+  return 3 * a.nchunk * nd + ((ll)a.nchunk * a.N + 3) / 4;
 }
 ll part_floats(const Plan& p) {
   const Args& a = p.a;
@@ -737,9 +753,9 @@ ll part_floats(const Plan& p) {
 void place(Plan& p, float* ws) {
   Args& a = p.a;
   const ll nd = (ll)a.N * a.D;
-  a.agg_a = ws;
-  a.agg_b = ws + a.nchunk * nd;
-  a.agg_cut = reinterpret_cast<unsigned char*>(ws + 2 * a.nchunk * nd);
+  a.agg_a = reinterpret_cast<double*>(ws);
+  a.agg_b = ws + 2 * a.nchunk * nd;
+  a.agg_cut = reinterpret_cast<unsigned char*>(ws + 3 * a.nchunk * nd);
   a.part = ws + agg_floats(p);
 }
 
@@ -828,6 +844,7 @@ int mjh_scan_forward(const mjh_scan_desc* d, void* stream) {
   if (int rc = make_plan(d, p)) return rc;
   if (!d->x || !d->gate || !d->h || !d->last) return refuse("scan forward: x, gate, h and last are needed");
   if (d->ws_bytes < 4 * agg_floats(p) || (agg_floats(p) && !d->ws)) return refuse("scan forward: workspace too small");
+  if (agg_floats(p) && !aligned(d->ws, 16)) return refuse("scan forward: the workspace must be aligned to 16 bytes");
   place(p, static_cast<float*>(d->ws));
   if (p.a.nchunk > 1)
     if (int rc = launch(kForwardAgg, p, *d, stream)) return rc;
@@ -840,6 +857,7 @@ int mjh_scan_backward(const mjh_scan_desc* d, void* stream) {
   if (!d->x || !d->gate || !d->kept) return refuse("scan backward: x, gate and the kept states are needed");
   const ll need = agg_floats(p) + part_floats(p);
   if (d->ws_bytes < 4 * need || (need && !d->ws)) return refuse("scan backward: workspace too small");
+  if (need && !aligned(d->ws, 16)) return refuse("scan backward: the workspace must be aligned to 16 bytes");
   place(p, static_cast<float*>(d->ws));
   if (p.a.nchunk > 1)
     if (int rc = launch(kBackwardAgg, p, *d, stream)) return rc;

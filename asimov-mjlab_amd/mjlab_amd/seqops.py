@@ -77,9 +77,7 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor | None =
   Channel ``d`` of row ``n`` uses gate ``d // (D // G)`` (one gate per channel, or one per head):
 
   * ``mode="blend"``: ``h_t = sigmoid(gate) h' + sigmoid(-gate) x_t``
-  * ``mode="decay"``: ``h_t = gate h' + x_t`` (any real gate; a long scan of few channels is cut into
-    chunks, over whose steps the product of the gates has to stay in float32's range, as that of gates
-    in [-1, 1] does, wherever a state comes in)
+  * ``mode="decay"``: ``h_t = gate h' + x_t`` (any real gate)
 
   with ``h' = 0`` where ``reset[t, n]`` (step t is the first of an episode: the ``dones`` of the env
   step that returned its observation), else the row's previous state; ``state`` (None: 0) precedes

@@ -681,7 +681,7 @@ const char* mjh_seq_last_error(void);
 /* Steps between the states that the forward pass keeps for the backward pass. */
 int mjh_scan_steps(void);
 
-/* Bytes of workspace for one forward (backward != 0: backward) call; -1: refused. */
+/* Bytes of workspace (16-byte aligned) for one forward (backward != 0: backward) call; -1: refused. */
 long long mjh_scan_workspace(const mjh_scan_desc* d, int backward);
 
 int mjh_scan_forward(const mjh_scan_desc* d, void* stream);

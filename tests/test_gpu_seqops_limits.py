@@ -5,9 +5,11 @@ import torch
 import torch.autograd.forward_ad as fwd
 
 from mjlab_amd import seqops
-from tests.test_gpu_seqops import rnd
+from tests import seq_ref
+from tests.test_gpu_seqops import check_scan, rnd, scan_inputs
 
 pytestmark = pytest.mark.gpu
+F32 = torch.float32
 
 
 # ---- forward-mode derivatives -------------------------------------------------------------
@@ -52,3 +54,57 @@ def test_forward_mode_over_a_gradient_is_refused():
     with fwd.dual_level():
       with pytest.raises(RuntimeError, match="forward-mode"):
         torch.autograd.grad(y, x, fwd.make_dual(up, torch.ones_like(up)))
+
+
+# ---- many chunks, and products of gates beyond float32 ---------------------------------------
+@pytest.mark.parametrize("mode", ["blend", "decay"])
+@pytest.mark.parametrize("t", [4096, 8192])
+@pytest.mark.parametrize("d,g", [(3, 3), (4, 2)])
+def test_scan_of_512_chunks(t, d, g, mode):
+  """The most chunks there are (512: 32 groups of 16, the last one full), with gates so near 1 that a state and a
+  gradient go through many groups; resets and lengths that end inside."""
+  x, gate, state, _, _, dh, dl = scan_inputs(t, 2, d, g, mode, F32, F32)
+  u = torch.rand(gate.shape, generator=torch.Generator().manual_seed(5)).cuda()
+  gate = 7 + 3 * u if mode == "blend" else 1 - 1e-3 * u
+  reset = torch.zeros(t, 2, dtype=torch.bool, device="cuda")
+  reset[t // 3 + 1, 0] = reset[t - 5, 0] = True
+  lengths = torch.tensor([t, t - t // 5], dtype=torch.int32, device="cuda")
+  check_scan((x, gate, state, None, None, dh, dl), mode)
+  check_scan((x, gate, state, reset, lengths, dh, dl), mode)
+
+
+@pytest.mark.parametrize("t,grow,gate_up,small", [
+  (8192, 256, 1.5, 1e-12),   # 16 chunks of 16 steps: 2^150 over a group, 2^9.4 over a chunk
+  (4096, 128, 2.5, 1e-20),   # 16 chunks of one block: 2^169
+  (8192, 16, 400.0, 1e-20),  # 2^138 inside one chunk
+  (4096, 8, 1e6, 1e-25),     # 2^159 inside one block
+])
+def test_small_states_under_growing_gates(t, grow, gate_up, small):
+  """A state that comes in small and grows by more than 2^128 stays finite, and so do the states, and (in the other
+  direction) the gradients, of all chunks around it; a gate of 0 among the growing ones erases what it should and no
+  more. Channel 0: growth; 1: a 0 inside the growth; 2: a 0 some steps behind it."""
+  x, _, state, _, _, dh, dl = scan_inputs(t, 1, 3, 3, "decay", F32, F32)
+  gate = torch.full((t, 1, 3), 0.9, device="cuda")
+  at = 4 * grow  # where a group, a chunk or a block begins
+  gate[at : at + grow] = gate_up
+  gate[at + grow - 3, 0, 1] = 0.0
+  gate[at + grow + 5, 0, 2] = 0.0
+  check_scan((x * small, gate, state * small, None, None, dh * small, dl * small), "decay")
+  reset = torch.zeros(t, 1, dtype=torch.bool, device="cuda")
+  reset[at + grow // 2] = True
+  check_scan((x * small, gate, state * small, reset, None, dh * small, dl * small), "decay")
+
+
+def test_growth_does_not_depend_on_the_plan():
+  """A row's result among few rows (steps in chunks) and among many (steps in one piece)."""
+  t, d, many = 512, 32, 2112  # 2,112 x 32 channels: no chunks
+  x, _, state, _, _, dh, dl = scan_inputs(t, 1, d, d, "decay", F32, F32)
+  gate = torch.full((t, 1, d), 0.9, device="cuda")
+  gate[128:256] = 2.2  # 2^145, in the join over one group of chunks
+  args = [v * 1e-12 for v in (x, state, dh, dl)]
+  few = check_scan((args[0], gate, args[1], None, None, args[2], args[3]), "decay")
+  with torch.no_grad():
+    h, last = seqops.gated_scan(args[0].repeat(1, many, 1), gate.repeat(1, many, 1), args[1].repeat(many, 1), mode="decay")
+  ref = seq_ref.scan(args[0], gate, args[1], mode="decay")
+  seq_ref.check(h[:, :1], *ref["h"], seq_ref.SCAN_ROUNDINGS, "h among many rows")
+  assert torch.isfinite(few[0]).all() and torch.isfinite(h).all() and torch.equal(last, last[:1].expand(many, d))

@@ -1,10 +1,14 @@
 """Policy-memory operators on the CPU at the limits of what their entry points take."""
 
+import ctypes
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
 
 from mjlab_amd import seqops
+from mjlab_amd.sim import native
+from tests import seq_ref
 
 
 def rnd(*shape, seed=0):
@@ -33,3 +37,15 @@ def test_forward_mode_on_the_cpu(name):
   # two float32 evaluations of at most 80 outputs, each of some 20 roundings, terms of size up to about 10
   assert abs(a - sum(t.sum() for t in terms)) <= 40 * 2.0**-24 * 10 * (sum(t.abs().sum() for t in terms) + 80)
   assert float(a.abs()) > 1e-3
+
+
+def test_scan_workspace_alignment():
+  """A workspace that a chunk's products could not be stored in is refused before any launch."""
+  lib, buf = native.lib(), torch.zeros(64)
+  d = seq_ref.ScanDesc()
+  d.x = d.gate = d.h = d.last = d.kept = buf.data_ptr() // 64 * 64
+  d.T, d.N, d.D, d.G = 100_000, 2, 6, 3
+  d.ws_bytes = max(lib.mjh_scan_workspace(ctypes.byref(d), back) for back in (0, 1))
+  d.ws = buf.data_ptr() // 64 * 64 + 8
+  for call in (lib.mjh_scan_forward, lib.mjh_scan_backward):
+    assert call(ctypes.byref(d), None) == 1 and b"aligned" in lib.mjh_seq_last_error()
