@@ -66,8 +66,10 @@ class PolicyMemory(nn.Module):
               lengths: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """(features (T, N, dim), last state (num_layers, N, dim)) of a rollout obs (T, N, obs_dim).
 
-    ``state``: the state before it (None: zeros; a copy of ``self.state`` taken when the rollout began).
-    ``reset`` (T, N) bool: obs[t] is the first of an episode. ``lengths`` (N,) int32: valid steps."""
+    ``state``: the state before it (None: zeros; else a copy of ``self.state`` from before ``step`` saw obs[0]).
+    ``reset`` (T, N) bool: obs[t] is the first of an episode. With the env wrapper, whose memory has seen the
+    current observations already, ``RslRlVecEnvWrapper.rollout_start`` gives the state and reset[0] before it.
+    ``lengths`` (N,) int32: valid steps."""
     if self.training and self.dropout:
       self.dropout_step.add_(1)
     last = []

@@ -11,9 +11,15 @@ step's outputs are also all-gathered across ranks (mjlab_amd.distributed).
 With ``memory`` (a PolicyMemory) set, the wrapper steps it on the ``memory_group``
 observations of every reset and env step, clears it at the envs that are done, and
 hands its features out as the observation ``"memory"`` next to the groups (not
-gathered: a learner on another rank forms them from the observations). The state
-before a rollout, which the learner's ``memory.forward`` needs, is
-``memory.state.clone()`` taken when the rollout begins.
+gathered: a learner on another rank forms them from the observations). A learner
+that stores each observation before the step that it is acted on with, from the
+current one on, asks ``rollout_start()`` for the state and the episode flags that
+precede it, before it steps on::
+
+  state, first = wrapper.rollout_start()
+  ...                                     # obs_0 .. obs_{T-1}, dones_0 .. dones_{T-1}
+  reset = torch.cat([first[None], dones[:-1].bool()])
+  features, _ = memory(obs, state, reset)
 """
 
 from __future__ import annotations
@@ -64,7 +70,12 @@ class RslRlVecEnvWrapper:
       self._gather = StepGather()
     self._modify_action_space()
     self.memory, self.memory_group = memory, memory_group
+    # of the last reset or step: the memory's features, the observations that they are of, and the state and the
+    # flags (obs is the first of an episode) from before these observations
     self._features: torch.Tensor | None = None
+    self._seen: torch.Tensor | None = None
+    self._state_before: torch.Tensor | None = None
+    self._first: torch.Tensor | None = None
     obs, _ = self.env.reset()
     self._restart_memory(obs)
 
@@ -107,16 +118,40 @@ class RslRlVecEnvWrapper:
     """Every env's memory empty, then the first observation in it."""
     if self.memory is not None:
       self.memory.reset_state(self.num_envs)
-      self._features = self.memory.step(obs[self.memory_group])
+      self._step_memory(obs, torch.ones(self.num_envs, dtype=torch.bool, device=self.memory.state.device))
+
+  def _step_memory(self, obs: dict, first: torch.Tensor) -> None:
+    state = self.memory.state
+    if self._state_before is None or (self._state_before.shape, self._state_before.device) != (state.shape, state.device):
+      with torch.inference_mode(False):  # a rollout's inference mode does not bind later ones to it
+        self._state_before, self._first = torch.empty_like(state), torch.empty_like(first)
+    self._state_before.copy_(state)
+    self._first.copy_(first)
+    self._seen = obs[self.memory_group].clone()
+    self._features = self.memory.step(self._seen, first)
+
+  def rollout_start(self) -> tuple[torch.Tensor, torch.Tensor]:
+    """(state, first): what ``memory.forward`` needs for a rollout whose obs[0] are the current observations.
+
+    ``state`` (num_layers, N, dim) is the memory before them, ``first`` (N,) bool says where they begin an episode
+    (the dones of the step that returned them): the rollout's ``reset[0]``. Copies; call it before the rollout's
+    first step."""
+    if self.memory is None:
+      raise ValueError("rollout_start: the wrapper has no memory")
+    return self._state_before.clone(), self._first.clone()
 
   def _with_memory(self, obs: dict) -> ObsDict:
     if self._features is not None:
-      obs = {**obs, "memory": self._features}
+      obs = {**obs, "memory": self._features.clone()}
     return ObsDict(obs, [self.num_envs])
 
   def get_observations(self) -> ObsDict:
-    # the memory's features are those of the last reset or step: looking again does not advance it
-    return self._with_memory(self.env.observation_manager.compute())
+    # the memory's features are those of the last reset or step: looking again does not advance it, and its group's
+    # observations, whose noise would be drawn anew, are those that it saw
+    obs = self.env.observation_manager.compute()
+    if self._seen is not None:
+      obs = {**obs, self.memory_group: self._seen.clone()}
+    return self._with_memory(obs)
 
   def reset(self):
     obs, extras = self.env.reset()
@@ -144,7 +179,7 @@ class RslRlVecEnvWrapper:
     if self._gather is not None:
       extras["gathered"] = self._gather(obs, rew, terminated, truncated)
     if self.memory is not None:  # a done env's obs is its next episode's first
-      self._features = self.memory.step(obs[self.memory_group], dones.bool())
+      self._step_memory(obs, dones.bool())
     return self._with_memory(obs), rew, dones, extras
 
   def close(self) -> None:
