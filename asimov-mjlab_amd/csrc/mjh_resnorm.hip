@@ -922,7 +922,7 @@ __global__ __launch_bounds__(256) void resnorm_join_scale(const Join j) {
 struct DropArgs {
   const void* x; ll xs;
   void* y; ll ysd;
-  ll rows; int cols;  // x rows of `cols` elements at stride xs (one row: flat)
+  ll rows, cols;  // x rows of `cols` elements at stride xs (one row: flat)
   ll count;
   Drop drop;
   mjh_i64* ctr_out;
@@ -1197,7 +1197,7 @@ int mjh_resnorm_backward(const mjh_resnorm_desc* d, void* stream) {
   return launched();
 }
 
-int mjh_dropout(const void* x, long long xs, void* y, long long ys, long long rows, int cols, int dtype, float scale,
+int mjh_dropout(const void* x, long long xs, void* y, long long ys, long long rows, long long cols, int dtype, float scale,
                 unsigned long long thr, unsigned long long seed, unsigned long long key, const mjh_i64* ctr,
                 mjh_i64* ctr_out, void* stream) {
   if (rows < 0 || cols < 0) return refuse("dropout: negative size");
@@ -1205,6 +1205,7 @@ int mjh_dropout(const void* x, long long xs, void* y, long long ys, long long ro
   if (thr > (1ull << 32)) return refuse("dropout: threshold above 2^32");
   if (rows == 0 || cols == 0) return 0;
   if (!x || !y) return refuse("dropout: x and y are needed");
+  if (rows > (1ll << 62) / cols) return refuse("dropout: more than 2^62 elements");
   DropArgs a;
   a.x = x; a.xs = xs; a.y = y; a.ysd = ys;
   a.count = rows * cols;

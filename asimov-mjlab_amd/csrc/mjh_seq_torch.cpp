@@ -324,20 +324,14 @@ Tensor dropout_run(const Tensor& x0, double scale, const Stream& r, const Tensor
   Tensor x = x0;
   ll rows = 1, cols = x.numel(), xs = 0;
   if (!x.is_contiguous()) {
-    if (x.dim() == 2 && x.stride(1) == 1 && x.stride(0) > 0 && x.size(1) <= 0x7fffffff) {
+    if (x.dim() == 2 && x.stride(1) == 1 && x.stride(0) > 0) {
       rows = x.size(0); cols = x.size(1); xs = x.stride(0);
     } else {
       x = x.contiguous();
     }
   }
-  if (rows == 1 && cols > 0x7fffffff) {  // rows of a length that fits an int, which number the elements the same
-    ll cut = 1 << 30;
-    while (cols % cut) cut >>= 1;
-    TORCH_CHECK(cut >= 1 << 10, "dropout: more than 2^31 elements must be a multiple of 1,024");
-    rows = cols / cut; cols = cut; xs = cut;
-  }
   Tensor y = at::empty(x.sizes(), x.options());
-  check(lib.dropout(x.data_ptr(), xs, y.data_ptr(), cols, rows, (int)cols, type_of(x), (float)scale, r.thr, r.seed, r.key,
+  check(lib.dropout(x.data_ptr(), xs, y.data_ptr(), cols, rows, cols, type_of(x), (float)scale, r.thr, r.seed, r.key,
                     static_cast<const mjh_i64*>(ptr(ctr)), static_cast<mjh_i64*>(ptr(ctr_out)), stream_of(x)),
         "mjh_dropout");
   return y;

@@ -20,7 +20,7 @@ PKG = Path(__file__).resolve().parents[1]
 # MJH_LIB selects an alternative build of the same ABI (e.g. the phase-timing
 # build libmjh_prof.so used by tools/phase_profile.py).
 LIB_PATH = Path(os.environ.get("MJH_LIB", str(PKG / "libmjh.so")))
-ABI_VERSION = 17
+ABI_VERSION = 18
 
 EXPORTS = (
   "mjh_abi_version",
@@ -233,7 +233,7 @@ def lib() -> ctypes.CDLL:
   L.mjh_scan_workspace.restype = L.mjh_resnorm_workspace.restype = ll
   for f in (L.mjh_scan_forward, L.mjh_scan_backward, L.mjh_scan_step, L.mjh_resnorm_forward, L.mjh_resnorm_backward):
     f.argtypes = [vp, vp]
-  L.mjh_dropout.argtypes = [vp, ll, vp, ll, ll, ci, ci, cf, u64, u64, u64, vp, vp, vp]
+  L.mjh_dropout.argtypes = [vp, ll, vp, ll, ll, ll, ci, cf, u64, u64, u64, vp, vp, vp]
   if L.mjh_abi_version() != ABI_VERSION:
     raise NativeLibraryError(f"libmjh ABI {L.mjh_abi_version()} != {ABI_VERSION}")
   if L.mjh_sizeof_model() != ctypes.sizeof(abi.model_struct()):

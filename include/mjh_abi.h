@@ -34,7 +34,7 @@ typedef long long mjh_i64;
 extern "C" {
 #endif
 
-#define MJH_ABI_VERSION 17
+#define MJH_ABI_VERSION 18
 
 /* efc_type codes (mjtConstraint) */
 #define MJH_CNSTR_FRICTION_DOF 1
@@ -751,7 +751,7 @@ int mjh_resnorm_backward(const mjh_resnorm_desc* d, void* stream);
  * (seed, key, *ctr) stream: word w = mix(base + (w + 1) 0x9e3779b97f4a7c15), base and
  * mix as for mjh_uniform_draws; it is kept iff those 32 bits are >= thr. The
  * gradient is the same call on dy with ctr = the ctr_out of the forward call. */
-int mjh_dropout(const void* x, long long xs, void* y, long long ys, long long rows, int cols, int dtype, float scale,
+int mjh_dropout(const void* x, long long xs, void* y, long long ys, long long rows, long long cols, int dtype, float scale,
                 unsigned long long thr, unsigned long long seed, unsigned long long key, const mjh_i64* ctr,
                 mjh_i64* ctr_out, void* stream);
 

@@ -9,7 +9,7 @@ from tests import seq_ref
 from tests.test_gpu_seqops import check_scan, rnd, scan_inputs
 
 pytestmark = pytest.mark.gpu
-F32 = torch.float32
+F32, BF16 = torch.float32, torch.bfloat16
 
 
 # ---- forward-mode derivatives -------------------------------------------------------------
@@ -108,3 +108,27 @@ def test_growth_does_not_depend_on_the_plan():
   ref = seq_ref.scan(args[0], gate, args[1], mode="decay")
   seq_ref.check(h[:, :1], *ref["h"], seq_ref.SCAN_ROUNDINGS, "h among many rows")
   assert torch.isfinite(few[0]).all() and torch.isfinite(h).all() and torch.equal(last, last[:1].expand(many, d))
+
+
+# ---- sizes beyond 2^31 -----------------------------------------------------------------------
+def test_dropout_of_an_odd_count_beyond_31_bits():
+  """(21,691,755, 99) and one row of 2^31 + 1: more than 2^31 - 1 elements, no multiple of 1,024; forward and gradient."""
+  for shape in ((21_691_755, 99), ((1 << 31) + 1,)):
+    count = 1
+    for k in shape:
+      count *= k
+    assert count > (1 << 31) - 1 and count % 1024
+    x = torch.ones(shape, dtype=BF16, device="cuda").requires_grad_()
+    y = seqops.dropout(x, 0.5, 1, 2)
+    assert y.shape == x.shape
+    flat = y.detach().view(-1)
+    base = seqops._mix64(torch.tensor([1], device="cuda") ^ seqops._mix64(
+      torch.tensor([2], device="cuda") ^ seqops._mix64(torch.tensor([seqops._signed(seqops._GOLDEN)], device="cuda"))))
+    for at in (0, (1 << 30) + 7, (1 << 31) - 64, count - 50):
+      i = torch.arange(at, min(at + 64, count), device="cuda")
+      z = seqops._mix64(base + ((i >> 1) + 1) * seqops._signed(seqops._GOLDEN))
+      keep = torch.where(i & 1 == 0, z >> 32 & 0xFFFFFFFF, z & 0xFFFFFFFF) >= 1 << 31
+      assert torch.equal(flat[i], keep.to(BF16) * 2), (shape, at)
+    (g,) = torch.autograd.grad(y, x, torch.ones_like(y))
+    assert torch.equal(g, y.detach())
+    del x, y, g, flat

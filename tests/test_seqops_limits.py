@@ -49,3 +49,12 @@ def test_scan_workspace_alignment():
   d.ws = buf.data_ptr() // 64 * 64 + 8
   for call in (lib.mjh_scan_forward, lib.mjh_scan_backward):
     assert call(ctypes.byref(d), None) == 1 and b"aligned" in lib.mjh_seq_last_error()
+
+
+def test_dropout_counts_in_64_bits():
+  """The entry point takes a row of any length; what no count holds is refused before any launch."""
+  lib = native.lib()
+  assert lib.mjh_dropout(1024, 0, None, 0, 1, (1 << 31) + 1, 0, 1.0, 0, 0, 0, None, None, None) == 1
+  assert b"needed" in lib.mjh_seq_last_error()
+  assert lib.mjh_dropout(1024, 0, 1024, 0, 1 << 40, 1 << 40, 0, 1.0, 0, 0, 0, None, None, None) == 1
+  assert b"2^62" in lib.mjh_seq_last_error()
