@@ -94,8 +94,15 @@ Tensor workspace(ll bytes, const char* what, const Tensor& like) {
   TORCH_CHECK(bytes >= 0, what, " refused: ", lib.last_error());
   return bytes ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor();
 }
+// What the memory holds is what the tensor says: views that negate (the imaginary part of a conjugate) are written out.
+Tensor plain(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+// contiguous, or not defined
+Tensor whole(const Tensor& t) { return t.defined() ? plain(t).contiguous() : t; }
 // neighbouring channels; a copy only where they are not
-Tensor unit(const Tensor& t) { return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+Tensor unit(const Tensor& t0) {
+  const Tensor t = plain(t0);
+  return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous();
+}
 
 // The gradients of a pass that has no second derivative: asking for one raises when it is formed, not before.
 variable_list once(variable_list grads) {
@@ -169,8 +176,7 @@ ScanOut scan_forward(const Tensor& x0, const Tensor& gate0, const Tensor& state0
                      int mode, bool keep) {
   c10::DeviceGuard guard(x0.device());
   const Tensor x = unit(x0), gate = unit(gate0);
-  const Tensor state = state0.defined() ? state0.contiguous() : state0;
-  const Tensor lengths = lengths0.defined() ? lengths0.contiguous() : lengths0;
+  const Tensor state = whole(state0), lengths = whole(lengths0);
   const auto t = x.size(0), n = x.size(1), d = x.size(2);
   ScanOut o;
   const auto f32 = x.options().dtype(at::kFloat);
@@ -207,8 +213,8 @@ struct Scan : torch::autograd::Function<Scan> {
     no_tangent("gated_scan's backward pass", {&grads[0], &grads[1]});
     c10::DeviceGuard guard(saved[0].device());
     const Tensor x = unit(saved[0]), gate = unit(saved[1]), reset = saved[2];
-    const Tensor lengths = saved[3].defined() ? saved[3].contiguous() : saved[3];
-    const Tensor dh = grads[0].defined() ? unit(grads[0]) : Tensor(), dlast = grads[1].defined() ? grads[1].contiguous() : Tensor();
+    const Tensor lengths = whole(saved[3]);
+    const Tensor dh = grads[0].defined() ? unit(grads[0]) : Tensor(), dlast = whole(grads[1]);
     const int64_t mode = ctx->saved_data["mode"].toInt();
     mjh_scan_desc s = scan_desc(x, gate, reset, lengths, (int)(mode & ~kHasState));
     s.kept = fptr(saved[4]);
@@ -274,8 +280,8 @@ py::object gated_step(const Tensor& x0, const Tensor& gate0, const Maybe& state_
   TORCH_CHECK(!wants_grad({&x0, &gate0, &state}),
               "gated_step: no gradients in the single-step form; use gated_scan, or torch.no_grad()");
   if (out.defined()) {
-    if (out.sizes() != state.sizes() || out.scalar_type() != at::kFloat || !out.is_contiguous() || out.device() != state.device())
-      refuse(name, ": out must be contiguous float32 of shape ", state.sizes(), " on ", state.device());
+    if (out.sizes() != state.sizes() || out.scalar_type() != at::kFloat || !out.is_contiguous() || out.is_neg() || out.device() != state.device())
+      refuse(name, ": out must be contiguous float32 (and no view that negates) of shape ", state.sizes(), " on ", state.device());
     TORCH_CHECK(!wants_grad({&out}), "gated_step: out requires a gradient");
     // what another thread may still read must not be written
     if (!(out.data_ptr() == state.data_ptr() && state.is_contiguous()) && overlap(out, state))
@@ -286,7 +292,7 @@ py::object gated_step(const Tensor& x0, const Tensor& gate0, const Maybe& state_
   no_tangent(name, {&x0, &gate0, &state, &out});
   c10::DeviceGuard guard(x0.device());
   if (!out.defined()) out = at::empty(state.sizes(), state.options());
-  if (!state.is_contiguous()) state = state.contiguous();
+  state = whole(state);
   const Tensor x = unit(x0), gate = unit(gate0);
   Tensor h = at::empty(x.sizes(), x.options());
   mjh_scan_desc s;
@@ -321,7 +327,7 @@ double drop_scale(double p) { return p < 1.0 ? 1.0 / (1.0 - p) : 0.0; }
 
 Tensor dropout_run(const Tensor& x0, double scale, const Stream& r, const Tensor& ctr, const Tensor& ctr_out) {
   c10::DeviceGuard guard(x0.device());
-  Tensor x = x0;
+  Tensor x = plain(x0);
   ll rows = 1, cols = x.numel(), xs = 0;
   if (!x.is_contiguous()) {
     if (x.dim() == 2 && x.stride(1) == 1 && x.stride(0) > 0) {
@@ -411,7 +417,7 @@ struct Rows {
     }
     return true;
   }
-  explicit Rows(const Tensor& t0) : t(t0) {
+  explicit Rows(const Tensor& t0) : t(plain(t0)) {
     if (!t.defined()) return;
     const ll dim = t.size(-1);
     if (t.is_contiguous()) {
@@ -425,14 +431,12 @@ struct Rows {
   }
 };
 
-Tensor flat(const Tensor& w) { return w.defined() ? w.contiguous() : w; }
-
 struct Operands {
   Rows y, r, gate;
   Tensor post_w, post_b, pre_w, pre_b, scale;
   Operands(const Tensor& y, const Tensor& r, const Tensor& gate, const Tensor& post_w, const Tensor& post_b, const Tensor& pre_w,
            const Tensor& pre_b, const Tensor& scale)
-      : y(y), r(r), gate(gate), post_w(flat(post_w)), post_b(flat(post_b)), pre_w(flat(pre_w)), pre_b(flat(pre_b)), scale(flat(scale)) {}
+      : y(y), r(r), gate(gate), post_w(whole(post_w)), post_b(whole(post_b)), pre_w(whole(pre_w)), pre_b(whole(pre_b)), scale(whole(scale)) {}
   mjh_resnorm_desc desc(const Norm& o, const Tensor& ctr) const {
     mjh_resnorm_desc d;
     std::memset(&d, 0, sizeof(d));

@@ -132,3 +132,33 @@ def test_dropout_of_an_odd_count_beyond_31_bits():
     (g,) = torch.autograd.grad(y, x, torch.ones_like(y))
     assert torch.equal(g, y.detach())
     del x, y, g, flat
+
+
+# ---- views that negate -------------------------------------------------------------------------
+def negated(*shape, seed=0):
+  """A view whose elements torch negates when it reads them: the memory holds the others' signs."""
+  v = torch.randn(*shape, dtype=torch.cfloat, generator=torch.Generator().manual_seed(seed)).cuda().conj().imag
+  assert v.is_neg()
+  return v
+
+
+def test_views_that_negate():
+  """One channel: neighbours need no stride of 1 and no copy is made for it."""
+  x, gate, state, up = negated(6, 3, 1), negated(6, 3, 1, seed=1), negated(3, 1, seed=2), negated(6, 3, 1, seed=3)
+  w = negated(1, seed=4)
+  plain = [v.resolve_neg().contiguous() for v in (x, gate, state, up, w)]
+
+  def run(x, gate, state, up, w):
+    leaves = [v.detach().requires_grad_() for v in (x, gate, state, w)]
+    h, last = seqops.gated_scan(*leaves[:3])
+    y = seqops.dropout(leaves[0], 0.3, 5)
+    s, n = seqops.residual_norm(leaves[0], leaves[1], gate=leaves[0], scale=leaves[3], post_weight=leaves[3], pre_weight=leaves[3])
+    grads = [g for o in (h, y, s, n) for g in torch.autograd.grad(o, leaves, up, allow_unused=True, retain_graph=True)]
+    with torch.no_grad():
+      one = seqops.gated_step(x[0], gate[0], state)
+    return [h, last, y, s, n, *one, *[g for g in grads if g is not None]]
+
+  for a, b in zip(run(x, gate, state, up, w), run(*plain)):
+    assert torch.equal(a, b)
+  with pytest.raises(ValueError, match="out must be"):
+    seqops.gated_step(plain[0][0], plain[1][0], plain[2], out=torch._neg_view(torch.zeros(3, 1, device="cuda")))
