@@ -53,7 +53,8 @@ class PolicyMemory(nn.Module):
     self.state: torch.Tensor | None = None  # (num_layers, N, dim) float32, what ``step`` carries
 
   def _blocks(self, obs: torch.Tensor, recur, p: float) -> torch.Tensor:
-    s, n = seqops.residual_norm(None, self.embed(obs), pre_weight=self.pre[0], norm=self.norm)
+    embedded = self.embed(obs.to(self.embed.weight.dtype))  # an env's observations are float32
+    s, n = seqops.residual_norm(None, embedded, pre_weight=self.pre[0], norm=self.norm)
     for i in range(self.num_layers):
       mixed = self.mix[i](n)
       value, gate, out_gate = mixed.split((self.dim, self.num_gates, self.dim), dim=-1)
