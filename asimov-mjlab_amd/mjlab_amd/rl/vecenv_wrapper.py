@@ -57,6 +57,12 @@ class ObsDict(dict):
 class RslRlVecEnvWrapper:
   def __init__(self, env: ManagerBasedRlEnv, clip_actions: float | None = None, gather: bool = False,
                memory: PolicyMemory | None = None, memory_group: str = "policy") -> None:
+    if memory is not None:
+      groups = env.observation_manager.active_terms
+      if "memory" in groups:  # the features would hide it
+        raise ValueError("the env's observation group 'memory' has the name of the memory's features")
+      if memory_group not in groups:
+        raise ValueError(f"the env has no group {memory_group!r} for the memory (groups: {', '.join(groups)})")
     self.env = env
     self.clip_actions = clip_actions
     self.num_envs = env.num_envs

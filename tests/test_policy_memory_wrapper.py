@@ -23,3 +23,14 @@ def test_memory_of_another_type_than_the_observations():
   # one layer: the rollout's rows and the step's are the same products, perhaps in another blocking: bfloat16 roundings
   # of the projections, the recurrence, the block's result and the features (values up to about 4)
   assert (a[0].float() - obs["memory"].float()).abs().max() <= 8 * 2.0**-8 * 4
+
+
+def test_a_group_of_the_features_name_is_refused():
+  def edit(cfg):
+    cfg.observations["memory"] = cfg.observations["critic"]
+
+  with pytest.raises(ValueError, match="'memory'"):
+    RslRlVecEnvWrapper(make_env(edit=edit), memory=PolicyMemory(99, dim=8))
+  assert set(RslRlVecEnvWrapper(make_env(edit=edit)).get_observations()) == {"policy", "critic", "memory"}
+  with pytest.raises(ValueError, match="no group 'other'"):
+    RslRlVecEnvWrapper(make_env(), memory=PolicyMemory(99, dim=8), memory_group="other")
