@@ -455,7 +455,7 @@ __global__ __launch_bounds__(threads_of(TPR)) void resnorm_backward(const Args a
         const float s = BLOCK ? __builtin_fmaf(scale[k], av[k] * u[k], r) : r;
         hat[k] = in[k] ? (s - pre_mean) * pre_rstd : 0.f;
         const float dn = (float)raw_dn[k];
-        sum[kPreW][k] += dn * hat[k];
+        if (in[k]) sum[kPreW][k] += dn * hat[k];
         if (BIAS) sum[kPreB][k] += in[k] ? dn : 0.f;
         const float dv = in[k] ? dn * pre_w[k] : 0.f;
         t[0] += dv * hat[k];

@@ -6,7 +6,7 @@ import torch.autograd.forward_ad as fwd
 
 from mjlab_amd import seqops
 from tests import seq_ref
-from tests.test_gpu_seqops import check_scan, rnd, scan_inputs
+from tests.test_gpu_seqops import call_norm, check_scan, norm_inputs, rnd, scan_inputs
 
 pytestmark = pytest.mark.gpu
 F32, BF16 = torch.float32, torch.bfloat16
@@ -162,3 +162,25 @@ def test_views_that_negate():
     assert torch.equal(a, b)
   with pytest.raises(ValueError, match="out must be"):
     seqops.gated_step(plain[0][0], plain[1][0], plain[2], out=torch._neg_view(torch.zeros(3, 1, device="cuda")))
+
+
+# ---- infinite gradients ------------------------------------------------------------------------
+@pytest.mark.parametrize("r", [5, 32, 70])
+@pytest.mark.parametrize("d", [3, 64, 99, 1000, 4097])
+def test_an_infinite_gradient_in_the_last_row(r, d):
+  """The weight's gradient of its column is infinite, as the sum over the rows is (not NaN: the last row counts once),
+  and no other column's changes."""
+  v, ds, dn = norm_inputs(r, d, F32, bias=True)
+  leaf = {k: None if t is None else t.detach().requires_grad_() for k, t in v.items()}
+  _, n = call_norm(leaf)
+  weights = [leaf["pre_w"], leaf["pre_b"]]
+  clean = torch.autograd.grad(n, weights, dn, retain_graph=True)
+  at, up = d // 2, dn.clone()
+  up[-1, at] = float("inf")
+  got = torch.autograd.grad(n, weights, up)
+  sign = torch.sign(seq_ref.resnorm(**{k: v[k] for k in ("gate", "scale", "post_w", "post_b")}, y=v["y"], r=v["res"],
+                                    pre_w=torch.ones(d), pre_b=torch.zeros(d))["n"][0][-1, at])
+  assert float(got[0][at]) == float(sign) * float("inf") and float(got[1][at]) == float("inf")
+  for a, b in zip(got, clean):
+    a[at] = b[at]
+    assert torch.equal(a, b)
