@@ -301,8 +301,8 @@ struct Row {
   }
 };
 
-// Bound by bytes (98,304 x 256 bfloat16, all parts: 54 us, 4.7 TB/s; 16,384 x 2,048: 49 us, 5.5 TB/s); for a few rows
-// by its chain of sums (16 x 1,000 float16: 4.5 us).
+// Bound by bytes (98,304 x 256 bfloat16, all parts: 60 us, 4.2 TB/s, 55 at the least; 16,384 x 2,048: 50 us, 5.3
+// TB/s); for a few rows by its chain of sums (16 x 1,000 float16: 5.0 us).
 template <class T, bool FULL, int TPR>
 __global__ __launch_bounds__(threads_of(TPR)) void resnorm_forward(const Args a) {
   typedef Row<T, FULL, TPR> R;
@@ -362,7 +362,8 @@ __global__ __launch_bounds__(threads_of(TPR)) void resnorm_forward(const Args a)
   }
 }
 
-// Bound by bytes (98,304 x 256 bfloat16, all parts: 83 us, 4.8 TB/s; 16,384 x 2,048 without gate: 86 us, 4.7 TB/s).
+// Bound by bytes (98,304 x 256 bfloat16, all parts: 88 us, 4.6 TB/s, 81 at the least; 16,384 x 2,048 without gate: 86
+// us, 4.7 TB/s).
 // BLOCK: there is a y (else only the norm before). BIAS: there are biases.
 template <class T, bool FULL, int TPR, bool BLOCK, bool BIAS>
 __global__ __launch_bounds__(threads_of(TPR)) void resnorm_backward(const Args a) {
@@ -930,7 +931,7 @@ struct DropArgs {
 
 // A stream of 16-byte pieces, V elements each; the words of a piece are one addition apart. A word costs two 64-bit
 // products, so a word for two elements keeps the arithmetic below the memory's time (at 50 million bfloat16
-// elements 40 us, 5.0 TB/s, about the rate of a copy of that size).
+// elements 42 us, 4.8 TB/s, 38.5 at the least; a copy of that size runs at 5.1, an element-wise torch kernel at 5.6).
 template <class T>
 __global__ __launch_bounds__(256) void dropout_flat(const DropArgs a) {
   constexpr int V = 16 / (int)sizeof(T);

@@ -339,7 +339,7 @@ __global__ __launch_bounds__(kBlock, GV == 2 ? 7 : 8) void scan_forward_agg(cons
   if (a.reset && w.d == 0) a.agg_cut[(ll)c * a.N + w.n] = cut;
 }
 
-// The outputs. Bound by bytes (24 x 4,096 x 256 bfloat16 with kept states: 38 us, 4.4 TB/s). AHEAD: loads of the next
+// The outputs. Bound by bytes (24 x 4,096 x 256 bfloat16 with kept states: 38 us, 4.5 TB/s). AHEAD: loads of the next
 // block under way while this one is worked on, for chunked launches; with a thread for every channel of many rows the
 // waves that its registers cost are worth more (24 x 4,096 x 256 bfloat16 without kept states: 33 us against 40).
 template <class T, class GT, int V, int GV, bool BLEND, bool AHEAD>
@@ -477,7 +477,7 @@ __device__ __forceinline__ int sum_over_lanes(float (&v)[kSteps], int lane, int 
 }
 
 // The gradients, steps in blocks from the last on: the states of a block forward from the kept one, then its steps
-// backward. Bound by bytes at the 3 waves a SIMD that its registers leave (24 x 4,096 x 256 bfloat16: 61 us, 4.3 TB/s).
+// backward. Bound by bytes at the 3 waves a SIMD that its registers leave (24 x 4,096 x 256 bfloat16: 59 us, 4.6 TB/s).
 // HEADS: dgate is summed over a head's lanes; lanes beside its channels take part with 0.
 template <class T, class GT, int V, int GV, bool BLEND, bool HEADS>
 __global__ __launch_bounds__(kBlock) void scan_backward(const Args a) {
@@ -621,7 +621,7 @@ __global__ __launch_bounds__(kBlock) void scan_join_heads(const Args a) {
 }
 
 // One step: out = a h' + ..., the state read from a.state and written to a.last (the same rows, or others). 4,096 x 256
-// bfloat16: 4.1 us, 3.6 TB/s; 1 x 128: 1.4 us.
+// bfloat16: 4.6 us, 3.2 TB/s; 1 x 128: 1.8 us.
 template <class T, class GT, int V, int GV, bool BLEND>
 __global__ __launch_bounds__(kBlock) void scan_step(const Args a) {
   const Where w = flat_where<V>(a);

@@ -96,7 +96,7 @@ __device__ __forceinline__ void store_loose(T* p, const float (&f)[V]) {
 
 // Waits for the loads issued so far. Before a loop that keeps a block of loads under way: a load of the first block
 // that may still be under way at the loop's entry costs a wait for every load at its use in each turn (scan, backward,
-// 16,384 x 2,048 bfloat16: 44 us, 47 so; norm's columns, 2,048 x 8,192: 56, 60).
+// 16,384 x 2,048 bfloat16: 43 us, 47 so; norm's columns, 2,048 x 8,192: 56, 60).
 __device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt 0; the others untouched
 
 inline bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }

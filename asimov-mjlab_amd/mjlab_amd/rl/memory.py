@@ -25,7 +25,9 @@ class PolicyMemory(nn.Module):
   divisor of ``dim``; default one per channel) and an output gate; the recurrence's result is
   projected, normed, gated, scaled and added to the residual stream. ``dropout`` acts on the blocks'
   results in training mode, drawn from (``seed``, layer, a device counter that each training
-  ``forward`` advances), so a captured training step drops anew at every replay."""
+  ``forward`` advances), so a captured training step drops anew at every replay. Ranks of one job draw the
+  same masks unless each has its own ``seed``; under activation checkpointing, whose second forward would
+  draw others than the first, leave ``dropout`` 0."""
 
   def __init__(self, obs_dim: int, dim: int = 256, num_layers: int = 2, num_gates: int | None = None, norm: str = "rms",
                dropout: float = 0.0, seed: int = 0, device=None, dtype: torch.dtype = torch.float32) -> None:
